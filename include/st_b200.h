@@ -356,6 +356,88 @@ ST_API st_status st_knn_search_sharded(st_handle *h, const uint8_t *codes, const
                                        int32_t prec, int64_t index_base, void *comm, float *out_scores,
                                        int64_t *out_ids);
 
+/* ---- token generation: a 4-bit paged cache, attention over it, logits ------ */
+/* The cache: data, device bytes [n_pages][kv_heads][page / 16][16 d + 128 d / group],
+ * 16-byte aligned; page a multiple of 16 up to 1024, d 64 or 128, group (the
+ * channels that share a scale) 32, 64 or 128 and at most d.  Slot s is token
+ * s % page of page s / page.  A tile of 16 tokens of one head holds key codes
+ * [d / group][16][group / 2] (channel 2b of the group in the low half of byte
+ * b), value codes [d / 2][16] (channel 2p in the low half; token t in column
+ * 4 ((t & 7) >> 1) + 2 (t & 1) + (t >> 3)), then f16 {scale, zero} pairs
+ * [d / group][16] of the keys and of the values.  A code c stands for
+ * c * scale + zero.  Device arrays throughout; element types by dtype
+ * (st_dtype).  None of these has a counterpart in the reference, whose
+ * sequences are at most 256 tokens and always run whole. */
+
+/* Appends n tokens: k, v [n, kv_heads, d] (rows of d contiguous elements,
+ * k_token / k_head elements between tokens / heads) go to slots (int64 [n], all
+ * different; negative: the token is left out).  rotary > 0 (even, at most d):
+ * the first `rotary` channels of the keys -- and of the queries, when q is not
+ * NULL: [n, heads, d] into q_out, packed -- are rotated by row positions[i]
+ * (int32 [n]) of cos, sin (f32 [n_positions, rotary / 2]), (a, b) -> (a cos -
+ * b sin, b cos + a sin) in f32, pairs (i, i + rotary / 2), or (2i, 2i + 1) with
+ * interleaved; queries whose slot is negative are rotated too.  Then, per
+ * group: zero = f16(min), scale = f16((max - zero) / 15), code = (x - zero) /
+ * scale to the nearest of 0 .. 15; x is clamped to +-65504 and NaN read as 0.
+ * A slot at or past n_pages * page, or a position outside [0, n_positions),
+ * leaves the token out and gives ST_INVALID_ARG at the next st_sync. */
+ST_API st_status st_kv4_append(st_handle *h, void *data, int64_t n_pages, int32_t page, int32_t kv_heads,
+                               int32_t d, int32_t group, const void *k, int64_t k_token, int64_t k_head,
+                               const void *v, int64_t v_token, int64_t v_head, const int64_t *slots, int64_t n,
+                               const void *q, int64_t q_token, int64_t q_head, void *q_out, int32_t heads,
+                               const float *cos, const float *sin, const int32_t *positions, int64_t n_positions,
+                               int32_t rotary, int32_t interleaved, int32_t dtype);
+/* k, v [n, kv_heads, d] (packed) = the values of the cache's slots[i]; zeros
+ * for a negative slot, and for one past the cache (ST_INVALID_ARG at the next
+ * st_sync). */
+ST_API st_status st_kv4_read(st_handle *h, const void *data, int64_t n_pages, int32_t page, int32_t kv_heads,
+                             int32_t d, int32_t group, const int64_t *slots, int64_t n, void *k, void *v,
+                             int32_t dtype);
+/* Attention of rows of queries over the cache.  Sequence b < batch has
+ * kv_len[b] keys, key j in slot (page j / page of pages[b * max_pages ...],
+ * j % page), and the rows q_start[b] .. q_start[b + 1] of q (int32 [batch + 1],
+ * ascending; NULL: row b), at most max_q of them, at positions kv_len[b] - its
+ * rows ... kv_len[b] - 1.  q [rows, heads, d] (q_token / q_head elements
+ * between tokens / heads); heads a multiple of kv_heads, query head h reads
+ * kv head h / (heads / kv_heads).  A row sees key j < kv_len[b], with causal
+ * only j <= its position, with window > 0 only j > position - window.
+ * o [rows, heads, d], packed; lse (f32 [rows, heads], or NULL) the natural-log
+ * sum of exp, with `one` (softmax1: a phantom zero logit) that term included.
+ * A row that sees no key gives 0 and -inf (softmax1: 0 and 0).  Entries of
+ * pages past a sequence's length are not read; slots past it may hold
+ * anything.  A length past max_pages * page, a page outside the cache or a row
+ * that belongs to no sequence is left out and gives ST_INVALID_ARG at the next
+ * st_sync.  workspace: device memory of st_kv4_attn_workspace's size, 16-byte
+ * aligned, written by this call alone while it runs; NULL: the handle's
+ * scratch. */
+ST_API st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, int64_t q_head, void *o, float *lse,
+                             const void *data, int64_t n_pages, int32_t page, int32_t heads, int32_t kv_heads,
+                             int32_t d, int32_t group, const int32_t *pages, int64_t max_pages,
+                             const int32_t *kv_len, const int32_t *q_start, int64_t batch, int64_t rows,
+                             int64_t max_q, float scale, int32_t causal, int32_t one, int32_t window, int32_t dtype,
+                             void *workspace, int64_t workspace_bytes);
+/* Bytes of the workspace for calls of these shapes. */
+ST_API st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int32_t heads,
+                                       int32_t kv_heads, int32_t d, int64_t *bytes);
+/* out [rows, vocab] (rows out_ld apart; may be logits itself) = logits (rows
+ * ld apart) after, in f32 and in this order: repetition, x / repetition[r] (x >
+ * 0) or x * repetition[r] for tokens in the row's history; - frequency[r] *
+ * times - presence[r] for tokens in the history after its first prompt[r];
+ * + the row's bias entries; -inf where the row's mask bit is 0.  The history is
+ * tokens[starts[r] .. starts[r + 1]) (int32; others than 0 .. vocab - 1 are
+ * skipped), the bias entries bias_starts[r] .. bias_starts[r + 1] of
+ * bias_tokens, bias_values (a token may occur twice: they are summed in order;
+ * tokens outside the vocabulary are skipped).  mask int32 [masks, (vocab + 31)
+ * / 32], bit v % 32 of word v / 32; row r uses mask mask_rows[r] (negative:
+ * none; at or past masks: none, and ST_INVALID_ARG at the next st_sync; NULL:
+ * mask r).  Every array but logits and out may be NULL (prompt NULL: 0). */
+ST_API st_status st_logits_adjust(st_handle *h, const void *logits, int64_t ld, void *out, int64_t out_ld,
+                                  int64_t rows, int64_t vocab, const int32_t *tokens, const int32_t *starts,
+                                  const int32_t *prompt, const float *repetition, const float *presence,
+                                  const float *frequency, const int32_t *bias_tokens, const float *bias_values,
+                                  const int32_t *bias_starts, const int32_t *mask, int64_t masks,
+                                  const int32_t *mask_rows, int32_t dtype);
+
 /* ---- kNN memory: 2-bit key scan fused with top-k ------------------------- */
 
 /* Ranking modes (src/gpu_step/knn.rs:5, :522-532, :855).

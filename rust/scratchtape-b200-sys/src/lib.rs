@@ -183,6 +183,25 @@ extern "C" {
                           n: i64, row_bytes: i64) -> st_status;
     pub fn st_knn_synth_keys(h: *mut st_handle, codes: *mut u8, scales: *mut f32, n: i64, dim: i32, seed: u64,
                              first_key: i64) -> st_status;
+    pub fn st_kv4_append(h: *mut st_handle, data: *mut c_void, n_pages: i64, page: i32, kv_heads: i32, d: i32,
+        group: i32, k: *const c_void, k_token: i64, k_head: i64, v: *const c_void, v_token: i64, v_head: i64,
+        slots: *const i64, n: i64, q: *const c_void, q_token: i64, q_head: i64, q_out: *mut c_void,
+        heads: i32, cos: *const f32, sin: *const f32, positions: *const i32, n_positions: i64, rotary: i32,
+        interleaved: i32, dtype: i32) -> st_status;
+    pub fn st_kv4_read(h: *mut st_handle, data: *const c_void, n_pages: i64, page: i32, kv_heads: i32, d: i32,
+        group: i32, slots: *const i64, n: i64, k: *mut c_void, v: *mut c_void, dtype: i32) -> st_status;
+    pub fn st_kv4_attn(h: *mut st_handle, q: *const c_void, q_token: i64, q_head: i64, o: *mut c_void,
+        lse: *mut f32, data: *const c_void, n_pages: i64, page: i32, heads: i32, kv_heads: i32, d: i32,
+        group: i32, pages: *const i32, max_pages: i64, kv_len: *const i32, q_start: *const i32, batch: i64,
+        rows: i64, max_q: i64, scale: f32, causal: i32, one: i32, window: i32, dtype: i32,
+        workspace: *mut c_void, workspace_bytes: i64) -> st_status;
+    pub fn st_kv4_attn_workspace(h: *mut st_handle, batch: i64, rows: i64, max_q: i64, heads: i32,
+        kv_heads: i32, d: i32, bytes: *mut i64) -> st_status;
+    pub fn st_logits_adjust(h: *mut st_handle, logits: *const c_void, ld: i64, out: *mut c_void, out_ld: i64,
+        rows: i64, vocab: i64, tokens: *const i32, starts: *const i32, prompt: *const i32,
+        repetition: *const f32, presence: *const f32, frequency: *const f32, bias_tokens: *const i32,
+        bias_values: *const f32, bias_starts: *const i32, mask: *const i32, masks: i64, mask_rows: *const i32,
+        dtype: i32) -> st_status;
 }
 
 /// A status and the handle's error text, as the reference's callers want a

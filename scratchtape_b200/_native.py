@@ -106,6 +106,14 @@ SIGNATURES = {
     "st_nccl_unique_id": (_st, [_vp]),
     "st_nccl_comm_init": (_st, [_i32, _i32, _vp, _i32, ctypes.POINTER(_vp)]),
     "st_nccl_comm_destroy": (_st, [_vp]),
+    "st_kv4_append": (_st, [_h, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp,
+                            _i64, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32]),
+    "st_kv4_read": (_st, [_h, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _i32]),
+    "st_kv4_attn": (_st, [_h, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp,
+                          _i64, _i64, _i64, _f32, _i32, _i32, _i32, _i32, _vp, _i64]),
+    "st_kv4_attn_workspace": (_st, [_h, _i64, _i64, _i64, _i32, _i32, _i32, ctypes.POINTER(_i64)]),
+    "st_logits_adjust": (_st, [_h, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                               _i64, _vp, _i32]),
     "st_avg_params": (_st, [_h, _vp, _i64, _vp]),
     "st_knn_search_sharded": (_st, [_h, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
 }

@@ -1,0 +1,65 @@
+// st_kv4.cuh -- the 4-bit paged cache: its layout, its quantiser's value form
+// and element conversions shared by the kernels that write and read it.
+//
+// data is [pages][kv_heads][page / 16][tile]; a tile is 16 tokens of one head:
+//   8 d bytes    key codes [group][token][G / 2], channel 2b of the group in
+//                the low half of byte b: a group's 16 rows lie one after the
+//                other, so eight rows read by a warp fill whole bank lines
+//   8 d bytes    value codes [d / 2][16], channel 2p in the low half of row
+//                p's bytes; token t in column kv4_col(t), the order in which
+//                one 32-bit word is one thread's part of a 16 x 16 operand
+//                of mma.sync (rows = channels, columns = tokens)
+//   64 d/G bytes key {scale, zero} [group][token], f16 pairs
+//   64 d/G bytes value {scale, zero}, likewise
+// A code c stands for c * scale + zero.  The tile is a multiple of 128 bytes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "st_internal.h"
+#include "st_ptx.cuh"
+
+namespace st {
+
+__host__ __device__ constexpr int kv4_tile_bytes(int d, int group) { return 16 * d + 128 * (d / group); }
+__host__ __device__ constexpr int kv4_val(int d) { return 8 * d; }
+__host__ __device__ constexpr int kv4_kmeta(int d) { return 16 * d; }
+__host__ __device__ constexpr int kv4_vmeta(int d, int group) { return 16 * d + 64 * (d / group); }
+// Column of token t (0..15) in a row of value codes.
+__host__ __device__ constexpr int kv4_col(int t) { return 4 * ((t & 7) >> 1) + 2 * (t & 1) + (t >> 3); }
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Checks the cache's shape; fills h's error and returns a status other than
+// ST_OK where it cannot be one.
+inline st_status kv4_check(st_handle *h, const char *who, const void *data, int64_t n_pages, int32_t page,
+                           int32_t kv_heads, int32_t d, int32_t group) {
+    if (!data || n_pages < 1 || kv_heads < 1) return h->fail(ST_INVALID_ARG, "%s: no cache", who);
+    if (reinterpret_cast<uintptr_t>(data) % 16 != 0)
+        return h->fail(ST_INVALID_ARG, "%s: the cache is not 16-byte aligned", who);
+    if (d != 64 && d != 128) return h->fail(ST_UNSUPPORTED_SHAPE, "%s: d = %d (64 or 128)", who, d);
+    if ((group != 32 && group != 64 && group != 128) || group > d)
+        return h->fail(ST_UNSUPPORTED_SHAPE, "%s: group = %d (32, 64 or 128, at most d)", who, group);
+    if (page < 16 || page > 1024 || page % 16 != 0)
+        return h->fail(ST_UNSUPPORTED_SHAPE, "%s: page = %d (a multiple of 16, at most 1024)", who, page);
+    if (n_pages > (1ll << 31) - 1 || kv_heads > 1024)
+        return h->fail(ST_UNSUPPORTED_SHAPE, "%s: too many pages or heads", who);
+    return ST_OK;
+}
+
+}  // namespace st
