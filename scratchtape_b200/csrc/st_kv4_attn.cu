@@ -4,6 +4,19 @@
 // j < len with j <= p (causal) and j > p - window (window > 0):
 //     x_j = scale q . k_j,  o = sum_j e^{x_j - m} v_j / (sum_j e^{x_j - m} [+ e^{-m}])
 // A row that sees nothing gives o = 0 and lse = -inf (softmax1: lse = 0).
+//
+// With codes c, scales s and zeros z by groups g of channels,
+//     q . k_j = sum_g s_jg (q_g . c_jg) + z_jg sum(q_g)
+//     o_g     = sum_j (p_j s_jg) c_jg + sum_j p_j z_jg
+// so the tensor cores multiply the codes themselves: a code in the low bits of
+// an f16 is the subnormal c 2^-24 (four bits further up, c 2^-20), exact, and
+// one AND makes two operands of mma.sync.  Codes are the 16-row operand (keys:
+// tokens x channels, values: channels x tokens), queries and weights the
+// 8-column one, so shared heads fill the columns and each cached byte is read
+// once, by one thread.
+#include <algorithm>
+#include <type_traits>
+
 #include "st_kv4.cuh"
 
 namespace {
@@ -17,99 +30,726 @@ struct AttnArgs {
     float *lse;
     const uint8_t *data;
     int64_t n_pages;
-    int page, heads, kv_heads;
+    int page, heads, kv_heads, share;
     const int32_t *pages;
     int64_t max_pages;
     const int32_t *kv_len, *q_start;
     int64_t batch, rows;
     int max_q;
-    float scale;
+    float scale_log2;  // scale * log2(e): scores are kept in units of log 2
     int causal, one, window;
+    int vec;           // rows of q start on 16-byte boundaries
+    float *work;       // pieces' partial results
     int *status;
 };
 
-// One warp per (row, head), one key at a time.
-template <typename T, int D, int G>
-__global__ void k_kv4_attn_rows(const AttnArgs a) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t w = blockIdx.x * static_cast<int64_t>(blockDim.x / 32) + threadIdx.x / 32;
-    if (w >= a.rows * a.heads) return;
-    const int64_t row = w / a.heads;
-    const int head = static_cast<int>(w % a.heads), kv_head = head / (a.heads / a.kv_heads), c = lane * E;
-    int64_t b = row, first = row, count = 1;
+// ---- which keys a sequence's rows see, and how the work is cut ---------------
+
+constexpr int UNIT = 32;     // keys of one step of a warp: two tiles
+constexpr int WARPS = 4;     // warps of a block; they take a piece's units in turn
+constexpr int MIN_UNITS = 4;  // units a block takes at least (one for each warp)
+
+struct Seq {
+    int64_t first;         // its first row
+    int count, len;        // rows, keys
+    int u0, units, blocks;  // units from u0 (at least one, where it has rows); blocks of RB rows of each head
+};
+
+// Sequence b, with lengths that do not fit left out (and reported).
+template <int RB>
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t b) {
+    Seq s;
+    s.first = b;
+    s.count = 1;
+    bool bad = false;
     if (a.q_start) {
-        int64_t lo = 0, hi = a.batch;  // the last b with q_start[b] <= row
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) / 2;
-            (a.q_start[mid] <= row ? lo : hi) = mid;
-        }
-        b = lo;
-        first = a.q_start[b];
-        count = a.q_start[b + 1] - first;
-        if (first > row || row >= first + count || count > a.max_q) {
-            if (lane == 0) set_status(a.status, DEV_BAD_ARG);
-            return;
+        const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
+        s.first = q0;
+        s.count = q1 - q0;
+        if (q0 < 0 || q1 < q0 || q1 > a.rows || s.count > a.max_q) {
+            s.count = 0;
+            bad = true;
         }
     }
-    int64_t len = a.kv_len[b];
-    if (len < 0 || len > a.max_pages * a.page) {
-        if (lane == 0) set_status(a.status, DEV_BAD_ARG);
-        len = len < 0 ? 0 : a.max_pages * a.page;
+    s.len = a.kv_len[b];
+    const int most = static_cast<int>(a.max_pages * a.page);
+    if (s.len < 0 || s.len > most) {
+        s.len = s.len < 0 ? 0 : most;
+        bad = true;
     }
-    const int64_t pos = len - count + (row - first);
-    const int64_t end = a.causal ? (pos + 1 < len ? pos + 1 : len) : len;
-    const int64_t begin = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    const T *q = static_cast<const T *>(a.q) + row * a.q_token + head * a.q_head + c;
-    float qf[E], o[E], m = a.one ? 0.0f : -INFINITY, l = a.one ? 1.0f : 0.0f;
+    if (bad) set_status(a.status, DEV_BAD_ARG);
+    const int begin = a.window > 0 ? max(0, s.len - s.count + 1 - a.window) : 0;
+    s.u0 = begin / UNIT;
+    s.units = max(1, (s.len + UNIT - 1) / UNIT - s.u0);
+    s.blocks = (s.count * a.share + RB - 1) / RB;
+    return s;
+}
+
+template <int RB>
+__device__ __forceinline__ int64_t weight_of(const AttnArgs &a, int64_t b) {
+    const Seq s = seq_of<RB>(a, b);
+    return static_cast<int64_t>(s.units) * s.blocks * a.kv_heads;
+}
+
+struct Cut {
+    int64_t total;  // units of all items (an item: a kv head's block of rows)
+    int64_t n;      // blocks that get some
+    int64_t at, b, base;  // where this one's part starts, in which sequence, and where that starts
+};
+
+// Units [total i / n, total (i + 1) / n) are block i's.  Every thread of the
+// block (of NW warps) calls it; smem holds 2 * NW + 2 int64.
+template <int RB, int NW>
+__device__ Cut cut_for(const AttnArgs &a, int64_t i, int64_t grid, int64_t *smem) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x / 32;
+    Cut c;
+    int64_t mine = 0, v = 0;
+    for (int64_t b = threadIdx.x; b < a.batch; b += blockDim.x) mine += v = weight_of<RB>(a, b);
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        qf[e] = to_f32(q[e]);
-        o[e] = 0.0f;
-    }
-    for (int64_t j = begin; j < end; j++) {
-        const int64_t p = a.pages[b * a.max_pages + j / a.page];
-        if (p < 0 || p >= a.n_pages) {
-            if (lane == 0) set_status(a.status, DEV_BAD_ARG);
-            continue;
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) smem[wid] = mine;
+    __syncthreads();
+    c.total = 0;
+    for (int w = 0; w < NW; w++) c.total += smem[w];
+    c.n = max(static_cast<int64_t>(1), min(grid, c.total / MIN_UNITS));
+    c.at = c.total * i / c.n;
+    int64_t carry = 0;
+    for (int64_t b0 = 0; b0 < a.batch; b0 += blockDim.x) {
+        const int64_t b = b0 + threadIdx.x;
+        if (a.batch > blockDim.x) v = b < a.batch ? weight_of<RB>(a, b) : 0;
+        int64_t incl = b < a.batch ? v : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
         }
-        const int off = static_cast<int>(j % a.page), r = off & 15;
-        const uint8_t *t =
-            a.data + ((p * a.kv_heads + kv_head) * (a.page / 16) + off / 16) * kv4_tile_bytes(D, G);
-        const float2 km =
-            __half22float2(*reinterpret_cast<const __half2 *>(t + kv4_kmeta(D) + ((c / G) * 16 + r) * 4));
-        const float2 vm =
-            __half22float2(*reinterpret_cast<const __half2 *>(t + kv4_vmeta(D, G) + ((c / G) * 16 + r) * 4));
-        const uint8_t *kr = t + (c / G) * 8 * G + r * (G / 2) + (c % G) / 2;
-        float x = 0.0f;
+        if (lane == 31) smem[NW + wid] = incl;
+        __syncthreads();
+        int64_t before = carry;
+        for (int w = 0; w < NW; w++) {
+            if (w < wid) before += smem[NW + w];
+            carry += smem[NW + w];
+        }
+        const int64_t end = before + incl, start = end - v;
+        if (b < a.batch && start <= c.at && c.at < end) {
+            smem[2 * NW] = b;
+            smem[2 * NW + 1] = start;
+        }
+        __syncthreads();
+    }
+    c.b = smem[2 * NW];
+    c.base = smem[2 * NW + 1];
+    return c;
+}
+
+// A partial result in the workspace: [RB][D] sums, then [RB] maxima, [RB] sums of weights.
+__host__ __device__ constexpr int64_t part_floats(int rb, int d) { return static_cast<int64_t>(rb) * (d + 2); }
+
+// ---- instructions -------------------------------------------------------------
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit elements across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+}
+
+// Words of a thread's part of a group's row of key codes: G / 32 of 32 bits.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
+    if constexpr (N == 1) {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    } else if constexpr (N == 2) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p);
+        w[0] = x.x, w[1] = x.y;
+    } else {
+        const uint4 x = *reinterpret_cast<const uint4 *>(p);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int vec, float (&x)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            x += qf[e] * fmaf(static_cast<float>(kr[e / 2] >> (e % 2 * 4) & 15), km.x, km.y);
+            for (int i = 0; i < 4; i++) {
+                T e[2];
+                memcpy(e, &w[i], 4);
+                x[2 * i] = to_f32(e[0]);
+                x[2 * i + 1] = to_f32(e[1]);
+            }
+        } else {
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-        x *= a.scale;
-        const float m2 = fmaxf(m, x), f = expf(m - m2), pr = expf(x - m2);
-        m = m2;
-        l = l * f + pr;
+            for (int i = 0; i < 2; i++) {
+                const float4 v = reinterpret_cast<const float4 *>(p)[i];
+                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+            }
+        }
+    } else {
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const uint32_t vb = t[kv4_val(D) + (c + e) / 2 * 16 + kv4_col(r)];
-            o[e] = o[e] * f + pr * fmaf(static_cast<float>(vb >> (e % 2 * 4) & 15), vm.x, vm.y);
+        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+    }
+}
+
+// ---- the kernel ---------------------------------------------------------------
+
+template <typename T, int D, int G, int NT>
+struct Shape {
+    static constexpr bool F32 = std::is_same<T, float>::value;
+    static constexpr int NG = D / G, RB = 8 * NT, TILE = kv4_tile_bytes(D, G), STAGE = 2 * TILE;
+    static constexpr int STAGES = D == 128 ? 3 : 5;
+    static constexpr int RING = STAGES * STAGE;  // bytes of a warp's ring; holds its [RB][D + 2] floats at the end
+    static_assert(RING >= RB * (D + 2) * 4, "a warp's result fits its ring");
+    static constexpr int SMEM = WARPS * RING;
+    static constexpr int PER_SM = NT == 1 ? (SMEM <= 56000 ? 4 : 3) : 2;  // blocks that an SM holds
+};
+
+// Writes four channels of row r's result and, once, its log-sum-exp.
+template <typename T, int D>
+__device__ __forceinline__ void finish(const AttnArgs &a, const Seq &s, int head, int r, int c, float4 o, float top,
+                                       float sum) {
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const int64_t out = (s.first + r / a.share) * a.heads + static_cast<int64_t>(head) * a.share + r % a.share;
+    T *dst = static_cast<T *>(a.o) + out * D + c;
+    dst[0] = from_f32<T>(o.x * inv), dst[1] = from_f32<T>(o.y * inv);
+    dst[2] = from_f32<T>(o.z * inv), dst[3] = from_f32<T>(o.w * inv);
+    if (a.lse && c == 0) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
+// One block: its part of the units, piece by piece (a piece: consecutive
+// units of one item).  Each warp has a ring of STAGES steps of two tiles that
+// bulk copies fill, and a running maximum, sum and result of its own; the
+// warps' results are joined at the end of a piece.  An item that one block
+// holds whole is written out; parts of one go to the workspace and are joined
+// by k_kv4_attn_join.
+template <typename T, int D, int G, int NT>
+__global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_attn(const AttnArgs a) {
+    using S = Shape<T, D, G, NT>;
+    constexpr int NG = S::NG, RB = S::RB, TILE = S::TILE, STAGES = S::STAGES, KS = G / 16, MT = D / 16;
+    constexpr int W = G / 32;          // words of a thread in a group's row of key codes
+    constexpr int QS = S::F32 ? 2 : 1;  // f32: queries and weights as two f16 terms, 22 bits
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t bars[WARPS][STAGES];
+    __shared__ int oks[WARPS][STAGES][2];
+    __shared__ int64_t scan[2 * WARPS + 2];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x / 32, g = lane >> 2, t = lane & 3;
+    uint8_t *ring = smem + wid * S::RING;
+    if (lane == 0)
+        for (int i = 0; i < STAGES; i++) mbar_init(&bars[wid][i], 1);
+    fence_mbar_init();
+    grid_dep_wait();
+    const Cut cut = cut_for<RB, WARPS>(a, blockIdx.x, gridDim.x, scan);
+    grid_dep_launch();
+    if (blockIdx.x >= cut.n) return;
+    const int64_t until = cut.total * (blockIdx.x + 1) / cut.n;
+    int64_t at = cut.at, b = cut.b, base = cut.base;
+    uint32_t phases = 0;  // bit i: the parity that stage i's next step completes
+    bool dead = false;
+    while (at < until) {
+        Seq s = seq_of<RB>(a, b);
+        for (int64_t w; at >= base + (w = static_cast<int64_t>(s.units) * s.blocks * a.kv_heads);) {
+            base += w;
+            s = seq_of<RB>(a, ++b);
+        }
+        const int item = static_cast<int>((at - base) / s.units), ua = static_cast<int>((at - base) % s.units);
+        const int ub = static_cast<int>(min(static_cast<int64_t>(s.units), ua + (until - at)));
+        const int head = item / s.blocks, row0 = item % s.blocks * RB;
+
+        // Queries: column n of the block is row row0 + n of (query, shared
+        // head).  Scaled by a power of two to just under 2^15 and held as f16
+        // (f32: two terms): exact for 16-bit types down to 2^-29 of the largest.
+        uint32_t qf[QS][NT][D / 16][2];
+        float c1[NT][2], c2[NT][NG][2];
+        int lo[NT][2], hi[NT][2];  // keys that columns 2t and 2t + 1 see
+        int all_lo = 0, all_hi = s.len;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = row0 + 8 * nt + g;
+            const bool real = r < s.count * a.share;
+            const T *q = static_cast<const T *>(a.q);
+            if (real)
+                q += (s.first + r / a.share) * a.q_token + (static_cast<int64_t>(head) * a.share + r % a.share) * a.q_head;
+            float x[NG][W][8], top = 0.0f, sum[NG];
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                sum[gr] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    if (real) {
+                        load8(q + gr * G + (t * W + w) * 8, a.vec, x[gr][w]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[gr][w][e] = 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        top = fmaxf(top, fabsf(x[gr][w][e]));
+                        sum[gr] += x[gr][w][e];
+                    }
+                }
+                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
+                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int up = top > 0.0f ? max(-100, min(100, 14 - static_cast<int>(__float_as_uint(top) >> 23) + 127)) : 0;
+            const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+            // a code is c 2^-24 (c 2^-20 in the upper nibbles: those channels take q / 16)
+            const float back = __uint_as_float(static_cast<uint32_t>(24 - up + 127) << 23) * a.scale_log2;
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                for (int w = 0; w < W; w++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float f = h ? mul * 0.0625f : mul;
+                            const float u = x[gr][w][2 * k + h] * f, v = x[gr][w][2 * k + h + 4] * f;
+                            const uint32_t p = pack2(u, v);
+                            qf[0][nt][gr * KS + 2 * w + k][h] = p;
+                            if constexpr (S::F32) {
+                                const float2 r2 = unpack2(p);
+                                qf[QS - 1][nt][gr * KS + 2 * w + k][h] = pack2(u - r2.x, v - r2.y);
+                            }
+                        }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                c1[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)
+                    c2[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], (2 * t + e) * 4) * a.scale_log2;
+                const int rr = min(row0 + 8 * nt + 2 * t + e, s.count * a.share - 1);
+                const int pos = s.len - s.count + rr / a.share;
+                hi[nt][e] = a.causal ? min(s.len, pos + 1) : s.len;
+                lo[nt][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+                all_lo = max(all_lo, lo[nt][e]);
+                all_hi = min(all_hi, hi[nt][e]);
+            }
+        }
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+
+        // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 0 and 1
+        // fetch the unit's two tiles; page numbers are loaded one step ahead.
+        const int n_units = !dead && ub - ua > wid ? (ub - ua - wid + WARPS - 1) / WARPS : 0;
+        const int32_t *table = a.pages + b * a.max_pages;
+        auto key_of = [&](int i) { return (s.u0 + ua + wid + i * WARPS) * UNIT + lane * 16; };
+        auto page_of = [&](int i) {  // of step i's tile `lane`
+            return lane < 2 && i < n_units && key_of(i) < s.len ? table[key_of(i) / a.page] : -1;
+        };
+        auto fetch = [&](int i, int stage, int page) {
+            const int key = key_of(i);
+            const bool ok = lane < 2 && page >= 0 && page < a.n_pages;
+            if (lane < 2 && key < s.len && !ok) set_status(a.status, DEV_BAD_ARG);
+            const uint32_t got = __ballot_sync(0xffffffffu, ok);
+            if (lane < 2) oks[wid][stage][lane] = ok;
+            if (lane == 0) mbar_arrive_expect_tx(&bars[wid][stage], __popc(got) * TILE);
+            __syncwarp();
+            if (ok) {
+                const int64_t tile = (static_cast<int64_t>(page) * a.kv_heads + head) * (a.page / 16) + key % a.page / 16;
+                bulk_load(ring + stage * S::STAGE + lane * TILE, a.data + tile * TILE, TILE, &bars[wid][stage]);
+            }
+        };
+        int next = page_of(0), issued = 0;
+        while (issued < STAGES - 1 && issued < n_units) {
+            const int page = next;
+            next = page_of(issued + 1);
+            fetch(issued, issued, page);
+            issued++;
+        }
+
+        float acc[NT][MT][4], l[NT][2], z[NT][NG][2], m[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                l[nt][e] = 0.0f;
+                m[nt][e] = -INFINITY;
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) z[nt][gr][e] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
+        }
+        int vexp = 0;  // f16 exponent of the largest value scale so far: weights are kept times 2^(29 - vexp)
+        int stage = 0;
+        for (int i = 0; i < n_units; i++) {
+            if (issued < n_units && !dead) {
+                const int page = next;
+                next = page_of(issued + 1);
+                fetch(issued, stage == 0 ? STAGES - 1 : stage - 1, page);
+                issued++;
+            }
+            if (i >= issued) break;
+            // a wait that runs out ends the loads; those in flight are still waited for
+            dead |= __any_sync(0xffffffffu, !mbar_wait(&bars[wid][stage], phases >> stage & 1, a.status, DEV_TIMEOUT_FULL));
+            phases ^= 1u << stage;
+            const uint8_t *base_t = ring + stage * S::STAGE;
+            const int key0 = (s.u0 + ua + wid + i * WARPS) * UNIT;
+            const int ok0 = oks[wid][stage][0], ok1 = oks[wid][stage][1];
+            const bool edge = key0 < all_lo || key0 + UNIT > all_hi || !ok0 || !ok1;
+
+            // scores, in units of log 2
+            float x[2][NT][4];
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++) {
+                const uint8_t *tp = base_t + tile * TILE;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[tile][nt][e] = 0.0f;
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    uint32_t wa[W], wb[W];
+                    load_words<W>(tp + gr * 8 * G + g * (G / 2) + t * (G / 8), wa);
+                    load_words<W>(tp + gr * 8 * G + (g + 8) * (G / 2) + t * (G / 8), wb);
+                    float raw[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) raw[nt][e] = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < W; w++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const uint32_t va = wa[w] >> (8 * k), vb = wb[w] >> (8 * k);
+                            const uint32_t a0 = va & 0x000f000fu, a1 = vb & 0x000f000fu, a2 = va & 0x00f000f0u,
+                                           a3 = vb & 0x00f000f0u;
+#pragma unroll
+                            for (int qs = QS - 1; qs >= 0; qs--)
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++)
+                                    mma_f16(raw[nt], a0, a1, a2, a3, qf[qs][nt][gr * KS + 2 * w + k][0],
+                                            qf[qs][nt][gr * KS + 2 * w + k][1]);
+                        }
+                    const uint32_t *meta = reinterpret_cast<const uint32_t *>(tp + kv4_kmeta(D)) + gr * 16 + g;
+                    const float2 ma = unpack2(meta[0]), mb = unpack2(meta[8]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float2 mm = e < 2 ? ma : mb;
+                            x[tile][nt][e] = fmaf(mm.x, raw[nt][e] * c1[nt][e & 1],
+                                                  fmaf(mm.y, c2[nt][gr][e & 1], x[tile][nt][e]));
+                        }
+                }
+            }
+            if (edge) {
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int key = key0 + tile * 16 + g + (e < 2 ? 0 : 8);
+                            if (key < lo[nt][e & 1] || key >= hi[nt][e & 1] || !(tile ? ok1 : ok0))
+                                x[tile][nt][e] = -INFINITY;
+                        }
+            }
+
+            // the values' scales and zeros; past the end they may be anything
+            float vs[2][NG][2], vz[2][NG][2];
+            int big = 0;
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t mm = *(reinterpret_cast<const uint32_t *>(base_t + tile * TILE + kv4_vmeta(D, G)) +
+                                        gr * 16 + g + 8 * h);
+                        if (edge && (key0 + tile * 16 + g + 8 * h >= s.len || !(tile ? ok1 : ok0))) mm = 0;
+                        big = max(big, static_cast<int>(mm & 0x7fffu));
+                        const float2 f = unpack2(mm);
+                        vs[tile][gr][h] = f.x;
+                        vz[tile][gr][h] = f.y;
+                    }
+
+            // running maximum; the result is rescaled where it or the scales' exponent grew
+            float fix[NT][2];
+            bool grew = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float top = fmaxf(fmaxf(x[0][nt][e], x[0][nt][e + 2]), fmaxf(x[1][nt][e], x[1][nt][e + 2]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float now = fmaxf(m[nt][e], top);
+                    grew |= now > m[nt][e];
+                    fix[nt][e] = now > m[nt][e] ? exp2_fast(m[nt][e] - now) : 1.0f;
+                    m[nt][e] = now;
+                }
+            const int ex = max(vexp, __reduce_max_sync(0xffffffffu, big) >> 10);
+            if (__any_sync(0xffffffffu, grew) || ex > vexp) {
+                const float down = __uint_as_float(static_cast<uint32_t>(127 + vexp - ex) << 23);
+                vexp = ex;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        l[nt][e] *= fix[nt][e];
+#pragma unroll
+                        for (int gr = 0; gr < NG; gr++) z[nt][gr][e] *= fix[nt][e];
+                    }
+#pragma unroll
+                    for (int i2 = 0; i2 < MT; i2++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[nt][i2][e] *= fix[nt][e & 1] * down;
+                }
+            }
+            // s 2^(29 - vexp) is below 2^15: f16 holds the weight times the scale to 11 bits
+            const float vmul = __uint_as_float(static_cast<uint32_t>(127 + 29 - vexp) << 23);
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++) {
+                const uint8_t *tp = base_t + tile * TILE;
+                uint32_t pf[QS][NT][NG][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float off = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+                        p[e] = exp2_fast(x[tile][nt][e] - off);
+                        l[nt][e & 1] += p[e];
+                    }
+#pragma unroll
+                    for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float sc = vs[tile][gr][h] * vmul;
+                            const float u = p[2 * h] * sc, v = p[2 * h + 1] * sc;
+                            const uint32_t w = pack2(u, v);
+                            pf[0][nt][gr][h] = transpose8(w);
+                            if constexpr (S::F32) {
+                                const float2 r2 = unpack2(w);
+                                pf[QS - 1][nt][gr][h] = transpose8(pack2(u - r2.x, v - r2.y));
+                            }
+                            z[nt][gr][0] = fmaf(p[2 * h], vz[tile][gr][h], z[nt][gr][0]);
+                            z[nt][gr][1] = fmaf(p[2 * h + 1], vz[tile][gr][h], z[nt][gr][1]);
+                        }
+                }
+                const uint32_t *vp = reinterpret_cast<const uint32_t *>(tp + kv4_val(D)) + lane;
+#pragma unroll
+                for (int i2 = 0; i2 < MT; i2++) {
+                    const uint32_t va = vp[i2 * 32], vb = va >> 8;
+                    const uint32_t a0 = va & 0x000f000fu, a1 = va & 0x00f000f0u, a2 = vb & 0x000f000fu,
+                                   a3 = vb & 0x00f000f0u;
+                    constexpr int PER = MT / NG;
+#pragma unroll
+                    for (int qs = QS - 1; qs >= 0; qs--)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            mma_f16(acc[nt][i2], a0, a1, a2, a3, pf[qs][nt][i2 / PER][0], pf[qs][nt][i2 / PER][1]);
+                }
+            }
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            __syncwarp();
+        }
+        // the next piece starts at stage 0 again: its parities are kept in `phases`
+
+        // Sums over the keys' lanes, then this warp's result into its ring.
+        float *mine = reinterpret_cast<float *>(ring);
+        const float unit = __uint_as_float(static_cast<uint32_t>(127 + 24 - 29 + vexp) << 23);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float ls = l[nt][e];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
+                const int row = 8 * nt + 2 * t + e;
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    float zs = z[nt][gr][e];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) zs += __shfl_xor_sync(0xffffffffu, zs, o);
+                    constexpr int PER = MT / NG;
+#pragma unroll
+                    for (int i2 = gr * PER; i2 < (gr + 1) * PER; i2++)
+                        *reinterpret_cast<float2 *>(mine + row * D + 16 * i2 + 2 * g) =
+                            make_float2(fmaf(acc[nt][i2][e], unit, zs), fmaf(acc[nt][i2][e + 2], unit * 0.0625f, zs));
+                }
+                if (g == 0) {
+                    mine[RB * D + row] = m[nt][e];
+                    mine[RB * D + RB + row] = ls;
+                }
+            }
+        __syncthreads();
+        const bool whole = ua == 0 && ub == s.units;
+        float *part = a.work + (2 * static_cast<int64_t>(blockIdx.x) + (at == cut.at ? 0 : 1)) * part_floats(RB, D);
+        for (int k = threadIdx.x; k < RB * (D / 4); k += WARPS * 32) {
+            const int row = k / (D / 4), c = k % (D / 4) * 4, r = row0 + row;
+            if (r >= s.count * a.share) continue;
+            float wm[WARPS], top = -INFINITY, sum = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++)
+                top = fmaxf(top, wm[w] = reinterpret_cast<const float *>(smem + w * S::RING)[RB * D + row]);
+            if (whole && a.one) top = fmaxf(top, 0.0f);
+            const float off = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float *src = reinterpret_cast<const float *>(smem + w * S::RING);
+                const float f = exp2_fast(wm[w] - off);
+                const float4 v = *reinterpret_cast<const float4 *>(src + row * D + c);
+                sum = fmaf(src[RB * D + RB + row], f, sum);
+                o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+            }
+            if (!whole) {
+                *reinterpret_cast<float4 *>(part + row * D + c) = o;
+                if (c == 0) {
+                    part[RB * D + row] = top;
+                    part[RB * D + RB + row] = sum;
+                }
+                continue;
+            }
+            if (a.one) sum += exp2_fast(-off);
+            finish<T, D>(a, s, head, r, c, o, top, sum);
+        }
+        fence_proxy_async_smem();  // the rings' next writers are bulk copies
+        __syncthreads();
+        at += ub - ua;
+    }
+}
+
+// Joins the pieces of the item that the start of part i + 1 cuts, for the
+// first such cut in the item.  Each thread adds up four channels of one row
+// over every SETS-th piece, eight loads in flight; the sets are then added in
+// order, so the result does not depend on timing.
+constexpr int JOIN = 512;
+template <typename T, int D, int RB>
+__global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a, int64_t grid) {
+    constexpr int VALS = RB * D / 4, SETS = JOIN / VALS;
+    __shared__ int64_t scan[2 * (JOIN / 32) + 2];
+    __shared__ float4 sums[SETS][VALS];
+    __shared__ float tops[SETS][RB], weights[SETS][RB];
+    grid_dep_wait();
+    const int64_t i = blockIdx.x + 1;
+    const Cut c = cut_for<RB, JOIN / 32>(a, i, grid, scan);
+    if (i >= c.n) return;
+    const Seq s = seq_of<RB>(a, c.b);
+    const int item = static_cast<int>((c.at - c.base) / s.units);
+    const int64_t start = c.base + static_cast<int64_t>(item) * s.units, end = start + s.units;
+    const int64_t before = c.total * (i - 1) / c.n;
+    if (start == c.at || before > start) return;
+    int64_t last = i;  // pieces: the last one of part i - 1, then the first ones of parts i .. last
+    {
+        // part j starts before `end`: total j / n < end
+        last = (end * c.n + c.total - 1) / c.total - 1;
+        while (last + 1 < c.n && c.total * (last + 1) / c.n < end) last++;
+        while (last > i && c.total * last / c.n >= end) last--;
+    }
+    const int pieces = static_cast<int>(last - i + 2);
+    const int64_t first = 2 * (i - 1) + (before == start ? 0 : 1);
+    const int head = item / s.blocks, row0 = item % s.blocks * RB;
+    const int set = threadIdx.x / VALS, row = threadIdx.x % VALS / (D / 4), ch = threadIdx.x % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = set; p0 < pieces; p0 += 8 * SETS) {
+        float pm[8], pl[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int p = p0 + k * SETS;
+            const float *src = a.work + (p == 0 ? first : 2 * (i + p - 1)) * part_floats(RB, D);
+            pm[k] = p < pieces ? src[RB * D + row] : -INFINITY;
+            pl[k] = p < pieces ? src[RB * D + RB + row] : 0.0f;
+            v[k] = p < pieces ? *reinterpret_cast<const float4 *>(src + row * D + ch) : make_float4(0, 0, 0, 0);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < 8; k++) now = fmaxf(now, pm[k]);
+        const float off = now == -INFINITY ? 0.0f : now, f = exp2_fast(top - off);
+        top = now;
+        sum *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float w = exp2_fast(pm[k] - off);
+            sum = fmaf(pl[k], w, sum);
+            o.x = fmaf(v[k].x, w, o.x), o.y = fmaf(v[k].y, w, o.y);
+            o.z = fmaf(v[k].z, w, o.z), o.w = fmaf(v[k].w, w, o.w);
         }
     }
-    T *out = static_cast<T *>(a.o) + w * D + c;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    sums[set][threadIdx.x % VALS] = o;
+    if (ch == 0) {
+        tops[set][row] = top;
+        weights[set][row] = sum;
+    }
+    __syncthreads();
+    const int r = row0 + row;
+    if (set > 0 || r >= s.count * a.share) return;
+    top = a.one ? 0.0f : -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; e++) out[e] = from_f32<T>(o[e] * inv);
-    if (a.lse && lane == 0) a.lse[w] = l > 0.0f ? m + logf(l) : -INFINITY;
+    for (int k = 0; k < SETS; k++) top = fmaxf(top, tops[k][row]);
+    const float off = top == -INFINITY ? 0.0f : top;
+    sum = a.one ? exp2_fast(-off) : 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < SETS; k++) {
+        const float w = exp2_fast(tops[k][row] - off);
+        const float4 v = sums[k][threadIdx.x];
+        sum = fmaf(weights[k][row], w, sum);
+        o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+    }
+    finish<T, D>(a, s, head, r, ch, o, top, sum);
+}
+
+// Eight columns (one group of 8 rows) unless a kv head has more rows than that.
+int columns_of(int64_t max_q, int share) { return max_q * share > 8 ? 2 : 1; }
+
+int64_t grid_of(const st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int kv_heads, int share, int nt,
+                int64_t max_keys, int per_sm) {
+    const int rb = 8 * nt;
+    const int64_t blocks = std::min((max_q * share + rb - 1) / rb * batch, (rows * share + rb - 1) / rb + batch);
+    const double units = static_cast<double>(blocks) * kv_heads * static_cast<double>((max_keys + UNIT - 1) / UNIT + 1);
+    const int64_t most = static_cast<int64_t>(h->num_sms) * per_sm;
+    return static_cast<int64_t>(std::max(1.0, std::min(static_cast<double>(most), units / MIN_UNITS + 1)));
+}
+
+template <typename T, int D, int G, int NT>
+st_status launch(st_handle *h, const AttnArgs &a) {
+    using S = Shape<T, D, G, NT>;
+    const int64_t grid = grid_of(h, a.batch, a.rows, a.max_q, a.kv_heads, a.share, NT, a.max_pages * a.page, S::PER_SM);
+    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_kv4_attn<T, D, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn<T, D, G, NT>, dim3(static_cast<unsigned>(grid)),
+                                         dim3(WARPS * 32), S::SMEM, a));
+    if (st_status s = st_after_launch(h, "k_kv4_attn"); s != ST_OK || grid == 1) return s;
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_join<T, D, S::RB>, dim3(static_cast<unsigned>(grid - 1)),
+                                         dim3(JOIN), 0, a, grid));
+    return st_after_launch(h, "k_kv4_attn_join");
 }
 
 template <typename T, int D, int G>
-st_status launch(st_handle *h, const AttnArgs &a) {
-    const int64_t blocks = (a.rows * a.heads + 3) / 4;
-    if (blocks > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_attn: too many rows");
-    k_kv4_attn_rows<T, D, G><<<static_cast<unsigned>(blocks), 128, 0, h->stream>>>(a);
-    return st_after_launch(h, "k_kv4_attn_rows");
+st_status by_columns(st_handle *h, const AttnArgs &a, int nt) {
+    return nt == 1 ? launch<T, D, G, 1>(h, a) : launch<T, D, G, 2>(h, a);
 }
 
 }  // namespace
@@ -117,8 +757,12 @@ st_status launch(st_handle *h, const AttnArgs &a) {
 extern "C" st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int32_t heads,
                                            int32_t kv_heads, int32_t d, int64_t *bytes) {
     if (!h) return ST_INVALID_ARG;
-    if (!bytes) return h->fail(ST_INVALID_ARG, "st_kv4_attn_workspace: null bytes");
-    *bytes = 0;
+    if (!bytes || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || batch < 0 || rows < 0 || max_q < 0 ||
+        (d != 64 && d != 128))
+        return h->fail(ST_INVALID_ARG, "st_kv4_attn_workspace: bad arguments");
+    const int nt = columns_of(max_q, heads / kv_heads);
+    const int64_t grid = grid_of(h, batch, rows, max_q, kv_heads, heads / kv_heads, nt, 1ll << 30, nt == 1 ? 4 : 2);
+    *bytes = 2 * grid * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
     return ST_OK;
 }
 
@@ -134,23 +778,36 @@ extern "C" st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, i
         return h->fail(ST_INVALID_ARG, "st_kv4_attn: bad arguments");
     if (heads < kv_heads || heads % kv_heads != 0)
         return h->fail(ST_INVALID_ARG, "st_kv4_attn: %d heads do not share %d", heads, kv_heads);
-    if (max_pages * page > 0x7fffffff || rows > 0x7fffffff || max_q > 0x7fffffff || batch > 0x7fffffff)
-        return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_attn: over 2^31 - 1 rows or keys");
+    if (max_pages * page > (1 << 30) || rows > (1 << 30) || max_q * (heads / kv_heads) > (1 << 30) ||
+        batch > (1 << 30))
+        return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_attn: over 2^30 rows or keys");
     if (!q_start && rows != batch)
         return h->fail(ST_INVALID_ARG, "st_kv4_attn: without q_start there is one row per sequence");
     if (rows == 0 || batch == 0) return ST_OK;
     if (!q || !o || (!pages && max_pages > 0) || !kv_len) return h->fail(ST_INVALID_ARG, "st_kv4_attn: null argument");
-    (void)workspace;
-    (void)workspace_bytes;
     cudaSetDevice(h->device);
+    if (!q_start) max_q = 1;
+    const int share = heads / kv_heads, nt = columns_of(max_q, share);
+    const int64_t grid = grid_of(h, batch, rows, max_q, kv_heads, share, nt, max_pages * page, nt == 1 ? 4 : 2);
+    const int64_t need = 2 * grid * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
+    if (workspace) {
+        if (workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+            return h->fail(ST_INVALID_ARG, "st_kv4_attn: the workspace needs %lld aligned bytes",
+                           static_cast<long long>(need));
+    } else if (!(workspace = st_scratch(h, SLOT_KV4, static_cast<size_t>(need)))) {
+        return ST_NO_MEMORY;
+    }
+    const int size = dtype == ST_F32 ? 4 : 2;
+    const int vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0;
     const AttnArgs a = {q, q_token, q_head, o, lse, static_cast<const uint8_t *>(data), n_pages, page, heads,
-                        kv_heads, pages, max_pages, kv_len, q_start, batch, rows, static_cast<int>(max_q), scale,
-                        causal, one, window, h->d_status};
-#define KV4_CASE(D_, G_)                                                       \
-    if (d == D_ && group == G_) {                                              \
-        if (dtype == ST_F32) return launch<float, D_, G_>(h, a);               \
-        if (dtype == ST_F16) return launch<__half, D_, G_>(h, a);              \
-        return launch<__nv_bfloat16, D_, G_>(h, a);                            \
+                        kv_heads, share, pages, max_pages, kv_len, q_start, batch, rows, static_cast<int>(max_q),
+                        scale * 1.44269504088896341f, causal, one, window, vec, static_cast<float *>(workspace),
+                        h->d_status};
+#define KV4_CASE(D_, G_)                                                               \
+    if (d == D_ && group == G_) {                                                      \
+        if (dtype == ST_F32) return by_columns<float, D_, G_>(h, a, nt);         \
+        if (dtype == ST_F16) return by_columns<__half, D_, G_>(h, a, nt);        \
+        return by_columns<__nv_bfloat16, D_, G_>(h, a, nt);                      \
     }
     KV4_CASE(64, 32)
     KV4_CASE(64, 64)
