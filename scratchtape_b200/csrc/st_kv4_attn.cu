@@ -36,6 +36,7 @@ struct AttnArgs {
     const int32_t *kv_len, *q_start;
     int64_t batch, rows;
     int max_q;
+    uint32_t page_magic;  // ceil(2^32 / (page / 16)), 0 for pages of one tile
     float scale_log2;  // scale * log2(e): scores are kept in units of log 2
     int causal, one, window;
     int vec;           // rows of q start on 16-byte boundaries
@@ -83,6 +84,12 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t b) {
     s.units = max(1, (s.len + UNIT - 1) / UNIT - s.u0);
     s.blocks = (s.count * a.share + RB - 1) / RB;
     return s;
+}
+
+// Keys [x, y) that row r of (query, shared head) of sequence s sees.
+__device__ __forceinline__ int2 seen_by(const AttnArgs &a, const Seq &s, int r) {
+    const int pos = s.len - s.count + min(r, s.count * a.share - 1) / a.share;
+    return make_int2(a.window > 0 ? max(0, pos - a.window + 1) : 0, a.causal ? min(s.len, pos + 1) : s.len);
 }
 
 template <int RB>
@@ -154,6 +161,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero.
+__device__ __forceinline__ void mma_f16_0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Transposes an 8 x 8 matrix of 16-bit elements across the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -253,12 +269,11 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
     constexpr int QS = S::F32 ? 2 : 1;  // f32: queries and weights as two f16 terms, 22 bits
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[WARPS][STAGES];
-    __shared__ int oks[WARPS][STAGES][2];
     __shared__ int64_t scan[2 * WARPS + 2];
     const int lane = threadIdx.x & 31, wid = threadIdx.x / 32, g = lane >> 2, t = lane & 3;
     uint8_t *ring = smem + wid * S::RING;
     if (lane == 0)
-        for (int i = 0; i < STAGES; i++) mbar_init(&bars[wid][i], 1);
+        for (int i = 0; i < STAGES; i++) mbar_init(&bars[wid][i], 2);
     fence_mbar_init();
     grid_dep_wait();
     const Cut cut = cut_for<RB, WARPS>(a, blockIdx.x, gridDim.x, scan);
@@ -279,12 +294,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
         const int head = item / s.blocks, row0 = item % s.blocks * RB;
 
         // Queries: column n of the block is row row0 + n of (query, shared
-        // head).  Scaled by a power of two to just under 2^15 and held as f16
-        // (f32: two terms): exact for 16-bit types down to 2^-29 of the largest.
+        // head).  Scaled by a power of two that takes the block's largest to
+        // just under 2^15 and held as f16 (f32: two terms): exact for 16-bit
+        // types but for elements below 2^-29 of the largest.
         uint32_t qf[QS][NT][D / 16][2];
-        float c1[NT][2], c2[NT][NG][2];
-        int lo[NT][2], hi[NT][2];  // keys that columns 2t and 2t + 1 see
+        float c2[NT][NG][2];
         int all_lo = 0, all_hi = s.len;
+        float xq[NT][NG][W][8], top_q = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const int r = row0 + 8 * nt + g;
@@ -292,33 +308,47 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
             const T *q = static_cast<const T *>(a.q);
             if (real)
                 q += (s.first + r / a.share) * a.q_token + (static_cast<int64_t>(head) * a.share + r % a.share) * a.q_head;
-            float x[NG][W][8], top = 0.0f, sum[NG];
+            float sum[NG];
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
                 sum[gr] = 0.0f;
 #pragma unroll
                 for (int w = 0; w < W; w++) {
+                    float(&x)[8] = xq[nt][gr][w];
                     if (real) {
-                        load8(q + gr * G + (t * W + w) * 8, a.vec, x[gr][w]);
+                        load8(q + gr * G + (t * W + w) * 8, a.vec, x);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[gr][w][e] = 0.0f;
+                        for (int e = 0; e < 8; e++) x[e] = 0.0f;
                     }
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        top = fmaxf(top, fabsf(x[gr][w][e]));
-                        sum[gr] += x[gr][w][e];
+                        top_q = fmaxf(top_q, fabsf(x[e]));
+                        sum[gr] += x[e];
                     }
                 }
                 sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
                 sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
             }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int up = top > 0.0f ? max(-100, min(100, 14 - static_cast<int>(__float_as_uint(top) >> 23) + 127)) : 0;
-            const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-            // a code is c 2^-24 (c 2^-20 in the upper nibbles: those channels take q / 16)
-            const float back = __uint_as_float(static_cast<uint32_t>(24 - up + 127) << 23) * a.scale_log2;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)
+                    c2[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], (2 * t + e) * 4) * a.scale_log2;
+                const int2 sees = seen_by(a, s, row0 + 8 * nt + 2 * t + e);
+                all_lo = max(all_lo, sees.x);
+                all_hi = min(all_hi, sees.y);
+            }
+        }
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        const int top_exp = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top_q)) >> 23);
+        const int up = top_exp > 0 ? max(-100, min(100, 14 + 127 - top_exp)) : 0;
+        const float up_mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+        // a code is c 2^-24 (c 2^-20 in the upper nibbles: those channels take q / 16)
+        const float c1 = __uint_as_float(static_cast<uint32_t>(24 - up + 127) << 23) * a.scale_log2;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int gr = 0; gr < NG; gr++)
 #pragma unroll
@@ -327,8 +357,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                     for (int k = 0; k < 2; k++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const float f = h ? mul * 0.0625f : mul;
-                            const float u = x[gr][w][2 * k + h] * f, v = x[gr][w][2 * k + h + 4] * f;
+                            const float f = h ? up_mul * 0.0625f : up_mul;
+                            const float u = xq[nt][gr][w][2 * k + h] * f, v = xq[nt][gr][w][2 * k + h + 4] * f;
                             const uint32_t p = pack2(u, v);
                             qf[0][nt][gr * KS + 2 * w + k][h] = p;
                             if constexpr (S::F32) {
@@ -336,59 +366,56 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                                 qf[QS - 1][nt][gr * KS + 2 * w + k][h] = pack2(u - r2.x, v - r2.y);
                             }
                         }
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                c1[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
-#pragma unroll
-                for (int gr = 0; gr < NG; gr++)
-                    c2[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], (2 * t + e) * 4) * a.scale_log2;
-                const int rr = min(row0 + 8 * nt + 2 * t + e, s.count * a.share - 1);
-                const int pos = s.len - s.count + rr / a.share;
-                hi[nt][e] = a.causal ? min(s.len, pos + 1) : s.len;
-                lo[nt][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-                all_lo = max(all_lo, lo[nt][e]);
-                all_hi = min(all_hi, hi[nt][e]);
-            }
-        }
-        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
-        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
 
-        // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 0 and 1
-        // fetch the unit's two tiles; page numbers are loaded one step ahead.
-        const int n_units = !dead && ub - ua > wid ? (ub - ua - wid + WARPS - 1) / WARPS : 0;
+        // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 2j and
+        // 2j + 1 find the two tiles of every 16th step from j on, so one pass
+        // of the warp serves 16 steps; the numbers of the 16 steps after
+        // those are already being loaded.
+        const int n_units = ub - ua > wid ? (ub - ua - wid + WARPS - 1) / WARPS : 0;
         const int32_t *table = a.pages + b * a.max_pages;
-        auto key_of = [&](int i) { return (s.u0 + ua + wid + i * WARPS) * UNIT + lane * 16; };
-        auto page_of = [&](int i) {  // of step i's tile `lane`
-            return lane < 2 && i < n_units && key_of(i) < s.len ? table[key_of(i) / a.page] : -1;
+        const int tile0 = (s.u0 + ua + wid) * 2 + (lane & 1) + (lane >> 1) * WARPS * 2;
+        const int n_tiles = (s.len + 15) / 16, page_tiles = a.page / 16;
+        // exact for tiles below 2^26 (the magic number is at most 63 / 2^32 of the quotient too large)
+        auto quot = [&](int tile) { return a.page_magic ? __umulhi(tile, a.page_magic) : tile; };
+        auto page_of = [&](int i16) {  // of this lane's tile among steps 16 i16 ...
+            const int tile = tile0 + i16 * 32 * WARPS;
+            return i16 * 16 + (lane >> 1) < n_units && tile < n_tiles ? table[quot(tile)] : -1;
         };
-        auto fetch = [&](int i, int stage, int page) {
-            const int key = key_of(i);
-            const bool ok = lane < 2 && page >= 0 && page < a.n_pages;
-            if (lane < 2 && key < s.len && !ok) set_status(a.status, DEV_BAD_ARG);
-            const uint32_t got = __ballot_sync(0xffffffffu, ok);
-            if (lane < 2) oks[wid][stage][lane] = ok;
-            if (lane == 0) mbar_arrive_expect_tx(&bars[wid][stage], __popc(got) * TILE);
-            __syncwarp();
-            if (ok) {
-                const int64_t tile = (static_cast<int64_t>(page) * a.kv_heads + head) * (a.page / 16) + key % a.page / 16;
-                bulk_load(ring + stage * S::STAGE + lane * TILE, a.data + tile * TILE, TILE, &bars[wid][stage]);
-            }
-        };
+        uint32_t oks = 0, oks_before = 0;  // lanes whose tile is there: of the fetched 16 steps, of those before
+        const uint8_t *src = nullptr;
         int next = page_of(0), issued = 0;
-        while (issued < STAGES - 1 && issued < n_units) {
-            const int page = next;
-            next = page_of(issued + 1);
-            fetch(issued, issued, page);
+        auto fetch = [&](int stage) {
+            if ((issued & 15) == 0) {
+                const int i16 = issued >> 4, tile = tile0 + i16 * 32 * WARPS, page = next;
+                const bool ok = page >= 0 && page < a.n_pages;
+                if (i16 * 16 + (lane >> 1) < n_units && tile < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
+                next = page_of(i16 + 1);
+                oks_before = oks;
+                oks = __ballot_sync(0xffffffffu, ok);
+                const uint32_t in_page = tile - quot(tile) * page_tiles;
+                src = a.data + ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + in_page) * TILE;
+            }
+            if (lane >> 1 == (issued & 15)) {  // each lane of the two: its tile, or none
+                const bool ok = !dead && (oks >> lane & 1u);
+                mbar_arrive_expect_tx(&bars[wid][stage], ok ? TILE : 0);
+                if (ok) bulk_load(ring + stage * S::STAGE + (lane & 1) * TILE, src, TILE, &bars[wid][stage]);
+            }
             issued++;
-        }
+        };
+        while (issued < STAGES - 1 && issued < n_units) fetch(issued);
 
-        float acc[NT][MT][4], l[NT][2], z[NT][NG][2], m[NT][2];
+        // Weights are 2^(x - ref).  With vexp the exponent of the largest
+        // value scale so far (below 2^(vexp - 14)), a weight times a scale
+        // stays below 2^15, so f16 holds it to 11 bits, while x - ref <= 29 -
+        // vexp; only past that is ref moved, to bring the largest to 21 - vexp,
+        // and what was summed so far rescaled.
+        float acc[NT][MT][4], l[NT][2], z[NT][NG][2], neg[NT][2];  // neg: -ref
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 l[nt][e] = 0.0f;
-                m[nt][e] = -INFINITY;
+                neg[nt][e] = 0.0f;
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) z[nt][gr][e] = 0.0f;
             }
@@ -397,43 +424,31 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
         }
-        int vexp = 0;  // f16 exponent of the largest value scale so far: weights are kept times 2^(29 - vexp)
+        int vexp = 0;
+        uint32_t seen = 0;  // columns (bit 2 nt + e) whose ref is set
+        bool fresh = true;  // some column's is not
         int stage = 0;
         for (int i = 0; i < n_units; i++) {
-            if (issued < n_units && !dead) {
-                const int page = next;
-                next = page_of(issued + 1);
-                fetch(issued, stage == 0 ? STAGES - 1 : stage - 1, page);
-                issued++;
-            }
-            if (i >= issued) break;
-            // a wait that runs out ends the loads; those in flight are still waited for
-            dead |= __any_sync(0xffffffffu, !mbar_wait(&bars[wid][stage], phases >> stage & 1, a.status, DEV_TIMEOUT_FULL));
+            if (issued < n_units) fetch(stage == 0 ? STAGES - 1 : stage - 1);
+            // a wait that runs out ends the loads: what is still in flight is waited for, the rest arrives empty
+            dead |= !mbar_wait(&bars[wid][stage], phases >> stage & 1, a.status, DEV_TIMEOUT_FULL);
             phases ^= 1u << stage;
             const uint8_t *base_t = ring + stage * S::STAGE;
             const int key0 = (s.u0 + ua + wid + i * WARPS) * UNIT;
-            const int ok0 = oks[wid][stage][0], ok1 = oks[wid][stage][1];
-            const bool edge = key0 < all_lo || key0 + UNIT > all_hi || !ok0 || !ok1;
+            const uint32_t there = ((i ^ (issued - 1)) & 16 ? oks_before : oks) >> (2 * (i & 15)) & 3u;
+            const bool edge = key0 < all_lo || key0 + UNIT > all_hi || there != 3u;
 
-            // scores, in units of log 2
+            // scores less ref, in units of log 2
             float x[2][NT][4];
 #pragma unroll
             for (int tile = 0; tile < 2; tile++) {
                 const uint8_t *tp = base_t + tile * TILE;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[tile][nt][e] = 0.0f;
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) {
                     uint32_t wa[W], wb[W];
                     load_words<W>(tp + gr * 8 * G + g * (G / 2) + t * (G / 8), wa);
                     load_words<W>(tp + gr * 8 * G + (g + 8) * (G / 2) + t * (G / 8), wb);
                     float raw[NT][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) raw[nt][e] = 0.0f;
 #pragma unroll
                     for (int w = 0; w < W; w++)
 #pragma unroll
@@ -444,89 +459,111 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
 #pragma unroll
                             for (int qs = QS - 1; qs >= 0; qs--)
 #pragma unroll
-                                for (int nt = 0; nt < NT; nt++)
-                                    mma_f16(raw[nt], a0, a1, a2, a3, qf[qs][nt][gr * KS + 2 * w + k][0],
-                                            qf[qs][nt][gr * KS + 2 * w + k][1]);
+                                for (int nt = 0; nt < NT; nt++) {
+                                    const uint32_t(&f)[2] = qf[qs][nt][gr * KS + 2 * w + k];
+                                    if (w == 0 && k == 0 && qs == QS - 1)
+                                        mma_f16_0(raw[nt], a0, a1, a2, a3, f[0], f[1]);
+                                    else
+                                        mma_f16(raw[nt], a0, a1, a2, a3, f[0], f[1]);
+                                }
                         }
                     const uint32_t *meta = reinterpret_cast<const uint32_t *>(tp + kv4_kmeta(D)) + gr * 16 + g;
-                    const float2 ma = unpack2(meta[0]), mb = unpack2(meta[8]);
+                    float2 ma = unpack2(meta[0]), mb = unpack2(meta[8]);
+                    ma.x *= c1, mb.x *= c1;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const float2 mm = e < 2 ? ma : mb;
-                            x[tile][nt][e] = fmaf(mm.x, raw[nt][e] * c1[nt][e & 1],
-                                                  fmaf(mm.y, c2[nt][gr][e & 1], x[tile][nt][e]));
+                            const float before = gr == 0 ? neg[nt][e & 1] : x[tile][nt][e];
+                            x[tile][nt][e] = fmaf(mm.x, raw[nt][e], fmaf(mm.y, c2[nt][gr][e & 1], before));
                         }
                 }
             }
-            if (edge) {
-#pragma unroll
-                for (int tile = 0; tile < 2; tile++)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int key = key0 + tile * 16 + g + (e < 2 ? 0 : 8);
-                            if (key < lo[nt][e & 1] || key >= hi[nt][e & 1] || !(tile ? ok1 : ok0))
-                                x[tile][nt][e] = -INFINITY;
-                        }
-            }
-
             // the values' scales and zeros; past the end they may be anything
-            float vs[2][NG][2], vz[2][NG][2];
-            int big = 0;
+            uint32_t vm[2][NG][2], big = 0;
 #pragma unroll
             for (int tile = 0; tile < 2; tile++)
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        uint32_t mm = *(reinterpret_cast<const uint32_t *>(base_t + tile * TILE + kv4_vmeta(D, G)) +
-                                        gr * 16 + g + 8 * h);
-                        if (edge && (key0 + tile * 16 + g + 8 * h >= s.len || !(tile ? ok1 : ok0))) mm = 0;
-                        big = max(big, static_cast<int>(mm & 0x7fffu));
-                        const float2 f = unpack2(mm);
-                        vs[tile][gr][h] = f.x;
-                        vz[tile][gr][h] = f.y;
+                        uint32_t &mm = vm[tile][gr][h];
+                        mm = *(reinterpret_cast<const uint32_t *>(base_t + tile * TILE + kv4_vmeta(D, G)) + gr * 16 +
+                               g + 8 * h);
                     }
-
-            // running maximum; the result is rescaled where it or the scales' exponent grew
-            float fix[NT][2];
-            bool grew = false;
+            if (edge) {
+                asm volatile("");  // a branch: few steps come here
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float top = fmaxf(fmaxf(x[0][nt][e], x[0][nt][e + 2]), fmaxf(x[1][nt][e], x[1][nt][e + 2]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float now = fmaxf(m[nt][e], top);
-                    grew |= now > m[nt][e];
-                    fix[nt][e] = now > m[nt][e] ? exp2_fast(m[nt][e] - now) : 1.0f;
-                    m[nt][e] = now;
-                }
-            const int ex = max(vexp, __reduce_max_sync(0xffffffffu, big) >> 10);
-            if (__any_sync(0xffffffffu, grew) || ex > vexp) {
-                const float down = __uint_as_float(static_cast<uint32_t>(127 + vexp - ex) << 23);
-                vexp = ex;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        l[nt][e] *= fix[nt][e];
+                        const int2 sees = seen_by(a, s, row0 + 8 * nt + 2 * t + e);
 #pragma unroll
-                        for (int gr = 0; gr < NG; gr++) z[nt][gr][e] *= fix[nt][e];
+                        for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int key = key0 + tile * 16 + g + 8 * h;
+                                if (key < sees.x || key >= sees.y || !(there >> tile & 1u))
+                                    x[tile][nt][2 * h + e] = -INFINITY;
+                            }
+                    }
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                    for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            if (key0 + tile * 16 + g + 8 * h >= s.len || !(there >> tile & 1u)) vm[tile][gr][h] = 0;
+            }
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)  // a scale is the low half, never negative
+                    big = __vimax3_s16x2(big, vm[tile][gr][0], vm[tile][gr][1]);
+            const int bexp = static_cast<int>(big & 0x7fffu) >> 10;
+            float most = x[0][0][0];
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) most = fmaxf(most, x[tile][nt][e]);
+            if (__any_sync(0xffffffffu, bexp > vexp || most > 29.0f - vexp) || fresh) {
+                const int grown = max(0, __reduce_max_sync(0xffffffffu, bexp) - vexp);
+                vexp += grown;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float fix[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float top = fmaxf(fmaxf(x[0][nt][e], x[0][nt][e + 2]), fmaxf(x[1][nt][e], x[1][nt][e + 2]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const uint32_t bit = 1u << (2 * nt + e);
+                        float move = top - (21 - vexp);
+                        if (seen & bit) move = fmaxf(move, static_cast<float>(grown));
+                        else if (top > -INFINITY) seen |= bit;
+                        else move = 0.0f;
+                        fix[e] = exp2_fast(-fmaxf(move, 0.0f));  // before the first key there is nothing to rescale
+                        neg[nt][e] -= move;
+                        l[nt][e] *= fix[e];
+#pragma unroll
+                        for (int gr = 0; gr < NG; gr++) z[nt][gr][e] *= fix[e];
+#pragma unroll
+                        for (int tile = 0; tile < 2; tile++) {
+                            x[tile][nt][e] -= move;
+                            x[tile][nt][e + 2] -= move;
+                        }
                     }
 #pragma unroll
                     for (int i2 = 0; i2 < MT; i2++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[nt][i2][e] *= fix[nt][e & 1] * down;
+                        for (int e = 0; e < 4; e++) acc[nt][i2][e] *= fix[e & 1];
                 }
+                fresh = __any_sync(0xffffffffu, seen != (1u << (2 * NT)) - 1);
             }
-            // s 2^(29 - vexp) is below 2^15: f16 holds the weight times the scale to 11 bits
-            const float vmul = __uint_as_float(static_cast<uint32_t>(127 + 29 - vexp) << 23);
 #pragma unroll
             for (int tile = 0; tile < 2; tile++) {
                 const uint8_t *tp = base_t + tile * TILE;
@@ -536,24 +573,23 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                     float p[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float off = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-                        p[e] = exp2_fast(x[tile][nt][e] - off);
+                        p[e] = exp2_fast(x[tile][nt][e]);
                         l[nt][e & 1] += p[e];
                     }
 #pragma unroll
                     for (int gr = 0; gr < NG; gr++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const float sc = vs[tile][gr][h] * vmul;
-                            const float u = p[2 * h] * sc, v = p[2 * h + 1] * sc;
+                            const float2 sz = unpack2(vm[tile][gr][h]);
+                            const float u = p[2 * h] * sz.x, v = p[2 * h + 1] * sz.x;
                             const uint32_t w = pack2(u, v);
                             pf[0][nt][gr][h] = transpose8(w);
                             if constexpr (S::F32) {
                                 const float2 r2 = unpack2(w);
                                 pf[QS - 1][nt][gr][h] = transpose8(pack2(u - r2.x, v - r2.y));
                             }
-                            z[nt][gr][0] = fmaf(p[2 * h], vz[tile][gr][h], z[nt][gr][0]);
-                            z[nt][gr][1] = fmaf(p[2 * h + 1], vz[tile][gr][h], z[nt][gr][1]);
+                            z[nt][gr][0] = fmaf(p[2 * h], sz.y, z[nt][gr][0]);
+                            z[nt][gr][1] = fmaf(p[2 * h + 1], sz.y, z[nt][gr][1]);
                         }
                 }
                 const uint32_t *vp = reinterpret_cast<const uint32_t *>(tp + kv4_val(D)) + lane;
@@ -577,7 +613,6 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
 
         // Sums over the keys' lanes, then this warp's result into its ring.
         float *mine = reinterpret_cast<float *>(ring);
-        const float unit = __uint_as_float(static_cast<uint32_t>(127 + 24 - 29 + vexp) << 23);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -595,10 +630,10 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
 #pragma unroll
                     for (int i2 = gr * PER; i2 < (gr + 1) * PER; i2++)
                         *reinterpret_cast<float2 *>(mine + row * D + 16 * i2 + 2 * g) =
-                            make_float2(fmaf(acc[nt][i2][e], unit, zs), fmaf(acc[nt][i2][e + 2], unit * 0.0625f, zs));
+                            make_float2(fmaf(acc[nt][i2][e], 0x1p24f, zs), fmaf(acc[nt][i2][e + 2], 0x1p20f, zs));
                 }
                 if (g == 0) {
-                    mine[RB * D + row] = m[nt][e];
+                    mine[RB * D + row] = ls > 0.0f || ls != ls ? -neg[nt][e] : -INFINITY;
                     mine[RB * D + RB + row] = ls;
                 }
             }
@@ -801,6 +836,7 @@ extern "C" st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, i
     const int vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0;
     const AttnArgs a = {q, q_token, q_head, o, lse, static_cast<const uint8_t *>(data), n_pages, page, heads,
                         kv_heads, share, pages, max_pages, kv_len, q_start, batch, rows, static_cast<int>(max_q),
+                        page == 16 ? 0u : static_cast<uint32_t>(((1ull << 32) + page / 16 - 1) / (page / 16)),
                         scale * 1.44269504088896341f, causal, one, window, vec, static_cast<float *>(workspace),
                         h->d_status};
 #define KV4_CASE(D_, G_)                                                               \
