@@ -98,15 +98,22 @@ __device__ __forceinline__ int64_t weight_of(const AttnArgs &a, int64_t b) {
     return static_cast<int64_t>(s.units) * s.blocks * a.kv_heads;
 }
 
+// a / b; 64-bit division only where it is needed (it costs about 100 instructions).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+
 struct Cut {
     int64_t total;  // units of all items (an item: a kv head's block of rows)
     int64_t n;      // blocks that get some
+    int64_t each, more;   // `each` units, the first `more` blocks one more
     int64_t at, b, base;  // where this one's part starts, in which sequence, and where that starts
+    __device__ int64_t start(int64_t i) const { return each * i + min(i, more); }
 };
 
-// Units [total i / n, total (i + 1) / n) are block i's.  Every thread of the
-// block (of NW warps) calls it; smem holds 2 * NW + 2 int64.
-template <int RB, int NW>
+// Units [start(i), start(i + 1)) are block i's.  Every thread of the
+// block calls it; smem holds 2 * WARPS + 2 int64.
+template <int RB>
 __device__ Cut cut_for(const AttnArgs &a, int64_t i, int64_t grid, int64_t *smem) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x / 32;
     Cut c;
@@ -117,9 +124,11 @@ __device__ Cut cut_for(const AttnArgs &a, int64_t i, int64_t grid, int64_t *smem
     if (lane == 0) smem[wid] = mine;
     __syncthreads();
     c.total = 0;
-    for (int w = 0; w < NW; w++) c.total += smem[w];
+    for (int w = 0; w < WARPS; w++) c.total += smem[w];
     c.n = max(static_cast<int64_t>(1), min(grid, c.total / MIN_UNITS));
-    c.at = c.total * i / c.n;
+    c.each = quotient(c.total, c.n);
+    c.more = c.total - c.each * c.n;
+    c.at = c.start(i);
     int64_t carry = 0;
     for (int64_t b0 = 0; b0 < a.batch; b0 += blockDim.x) {
         const int64_t b = b0 + threadIdx.x;
@@ -130,24 +139,33 @@ __device__ Cut cut_for(const AttnArgs &a, int64_t i, int64_t grid, int64_t *smem
             const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += t;
         }
-        if (lane == 31) smem[NW + wid] = incl;
+        if (lane == 31) smem[WARPS + wid] = incl;
         __syncthreads();
         int64_t before = carry;
-        for (int w = 0; w < NW; w++) {
-            if (w < wid) before += smem[NW + w];
-            carry += smem[NW + w];
+        for (int w = 0; w < WARPS; w++) {
+            if (w < wid) before += smem[WARPS + w];
+            carry += smem[WARPS + w];
         }
         const int64_t end = before + incl, start = end - v;
         if (b < a.batch && start <= c.at && c.at < end) {
-            smem[2 * NW] = b;
-            smem[2 * NW + 1] = start;
+            smem[2 * WARPS] = b;
+            smem[2 * WARPS + 1] = start;
         }
         __syncthreads();
     }
-    c.b = smem[2 * NW];
-    c.base = smem[2 * NW + 1];
+    c.b = smem[2 * WARPS];
+    c.base = smem[2 * WARPS + 1];
     return c;
 }
+
+// What a part leaves for the join, at the start of the workspace: the item
+// that its start cuts, if it is the first part to cut it.
+struct Note {
+    int pieces;  // of that item: in `slot`, then the first ones of this part and those after it (0: none)
+    int head, row0, rows;  // rows: of the sequence, times the shared heads
+    int64_t first, slot;
+};
+constexpr int NOTE_FLOATS = sizeof(Note) / 4;
 
 // A partial result in the workspace: [RB][D] sums, then [RB] maxima, [RB] sums of weights.
 __host__ __device__ constexpr int64_t part_floats(int rb, int d) { return static_cast<int64_t>(rb) * (d + 2); }
@@ -245,10 +263,10 @@ struct Shape {
 
 // Writes four channels of row r's result and, once, its log-sum-exp.
 template <typename T, int D>
-__device__ __forceinline__ void finish(const AttnArgs &a, const Seq &s, int head, int r, int c, float4 o, float top,
+__device__ __forceinline__ void finish(const AttnArgs &a, int64_t first, int head, int r, int c, float4 o, float top,
                                        float sum) {
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    const int64_t out = (s.first + r / a.share) * a.heads + static_cast<int64_t>(head) * a.share + r % a.share;
+    const int64_t out = (first + r / a.share) * a.heads + static_cast<int64_t>(head) * a.share + r % a.share;
     T *dst = static_cast<T *>(a.o) + out * D + c;
     dst[0] = from_f32<T>(o.x * inv), dst[1] = from_f32<T>(o.y * inv);
     dst[2] = from_f32<T>(o.z * inv), dst[3] = from_f32<T>(o.w * inv);
@@ -260,7 +278,7 @@ __device__ __forceinline__ void finish(const AttnArgs &a, const Seq &s, int head
 // bulk copies fill, and a running maximum, sum and result of its own; the
 // warps' results are joined at the end of a piece.  An item that one block
 // holds whole is written out; parts of one go to the workspace and are joined
-// by k_kv4_attn_join.
+// by k_kv4_attn_join, which finds them by the notes that the parts leave.
 template <typename T, int D, int G, int NT>
 __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_attn(const AttnArgs a) {
     using S = Shape<T, D, G, NT>;
@@ -276,10 +294,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
         for (int i = 0; i < STAGES; i++) mbar_init(&bars[wid][i], 2);
     fence_mbar_init();
     grid_dep_wait();
-    const Cut cut = cut_for<RB, WARPS>(a, blockIdx.x, gridDim.x, scan);
+    const Cut cut = cut_for<RB>(a, blockIdx.x, gridDim.x, scan);
     grid_dep_launch();
+    Note *note = reinterpret_cast<Note *>(a.work) + blockIdx.x;
+    if (threadIdx.x == 0) note->pieces = 0;
     if (blockIdx.x >= cut.n) return;
-    const int64_t until = cut.total * (blockIdx.x + 1) / cut.n;
+    const int64_t until = cut.start(blockIdx.x + 1);
     int64_t at = cut.at, b = cut.b, base = cut.base;
     uint32_t phases = 0;  // bit i: the parity that stage i's next step completes
     bool dead = false;
@@ -289,9 +309,55 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
             base += w;
             s = seq_of<RB>(a, ++b);
         }
-        const int item = static_cast<int>((at - base) / s.units), ua = static_cast<int>((at - base) % s.units);
+        const int item = static_cast<int>(quotient(at - base, s.units));
+        const int ua = static_cast<int>(at - base - static_cast<int64_t>(item) * s.units);
         const int ub = static_cast<int>(min(static_cast<int64_t>(s.units), ua + (until - at)));
         const int head = item / s.blocks, row0 = item % s.blocks * RB;
+        if (at == cut.at && ua > 0 && threadIdx.x == 0) {
+            const int64_t start = at - ua, before = cut.start(blockIdx.x - 1);
+            int64_t last = blockIdx.x;
+            while (last + 1 < cut.n && cut.start(last + 1) < start + s.units) last++;
+            if (before <= start)
+                *note = Note{static_cast<int>(last - blockIdx.x) + 2, head, row0, s.count * a.share, s.first,
+                             2 * (static_cast<int64_t>(blockIdx.x) - 1) + (before == start ? 0 : 1)};
+        }
+
+        // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 2j and
+        // 2j + 1 find the two tiles of every 16th step from j on, so one pass
+        // of the warp serves 16 steps; the numbers of the 16 steps after
+        // those are already being loaded.
+        const int n_units = ub - ua > wid ? (ub - ua - wid + WARPS - 1) / WARPS : 0;
+        const int32_t *table = a.pages + b * a.max_pages;
+        const int tile0 = (s.u0 + ua + wid) * 2 + (lane & 1) + (lane >> 1) * WARPS * 2;
+        const int n_tiles = (s.len + 15) / 16, page_tiles = a.page / 16;
+        // exact for tiles below 2^26 (the magic number is at most 63 / 2^32 of the quotient too large)
+        auto quot = [&](int tile) { return a.page_magic ? __umulhi(tile, a.page_magic) : tile; };
+        auto page_of = [&](int i16) {  // of this lane's tile among steps 16 i16 ...
+            const int tile = tile0 + i16 * 32 * WARPS;
+            return i16 * 16 + (lane >> 1) < n_units && tile < n_tiles ? table[quot(tile)] : -1;
+        };
+        uint32_t oks = 0, oks_before = 0;  // lanes whose tile is there: of the fetched 16 steps, of those before
+        const uint8_t *src = nullptr;
+        int next = page_of(0), issued = 0;
+        auto fetch = [&](int stage) {
+            if ((issued & 15) == 0) {
+                const int i16 = issued >> 4, tile = tile0 + i16 * 32 * WARPS, page = next;
+                const bool ok = page >= 0 && page < a.n_pages;
+                if (i16 * 16 + (lane >> 1) < n_units && tile < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
+                next = page_of(i16 + 1);
+                oks_before = oks;
+                oks = __ballot_sync(0xffffffffu, ok);
+                const uint32_t in_page = tile - quot(tile) * page_tiles;
+                src = a.data + ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + in_page) * TILE;
+            }
+            if (lane >> 1 == (issued & 15)) {  // each lane of the two: its tile, or none
+                const bool ok = !dead && (oks >> lane & 1u);
+                mbar_arrive_expect_tx(&bars[wid][stage], ok ? TILE : 0);
+                if (ok) bulk_load(ring + stage * S::STAGE + (lane & 1) * TILE, src, TILE, &bars[wid][stage]);
+            }
+            issued++;
+        };
+        while (issued < STAGES - 1 && issued < n_units) fetch(issued);
 
         // Queries: column n of the block is row row0 + n of (query, shared
         // head).  Scaled by a power of two that takes the block's largest to
@@ -366,43 +432,6 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                                 qf[QS - 1][nt][gr * KS + 2 * w + k][h] = pack2(u - r2.x, v - r2.y);
                             }
                         }
-
-        // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 2j and
-        // 2j + 1 find the two tiles of every 16th step from j on, so one pass
-        // of the warp serves 16 steps; the numbers of the 16 steps after
-        // those are already being loaded.
-        const int n_units = ub - ua > wid ? (ub - ua - wid + WARPS - 1) / WARPS : 0;
-        const int32_t *table = a.pages + b * a.max_pages;
-        const int tile0 = (s.u0 + ua + wid) * 2 + (lane & 1) + (lane >> 1) * WARPS * 2;
-        const int n_tiles = (s.len + 15) / 16, page_tiles = a.page / 16;
-        // exact for tiles below 2^26 (the magic number is at most 63 / 2^32 of the quotient too large)
-        auto quot = [&](int tile) { return a.page_magic ? __umulhi(tile, a.page_magic) : tile; };
-        auto page_of = [&](int i16) {  // of this lane's tile among steps 16 i16 ...
-            const int tile = tile0 + i16 * 32 * WARPS;
-            return i16 * 16 + (lane >> 1) < n_units && tile < n_tiles ? table[quot(tile)] : -1;
-        };
-        uint32_t oks = 0, oks_before = 0;  // lanes whose tile is there: of the fetched 16 steps, of those before
-        const uint8_t *src = nullptr;
-        int next = page_of(0), issued = 0;
-        auto fetch = [&](int stage) {
-            if ((issued & 15) == 0) {
-                const int i16 = issued >> 4, tile = tile0 + i16 * 32 * WARPS, page = next;
-                const bool ok = page >= 0 && page < a.n_pages;
-                if (i16 * 16 + (lane >> 1) < n_units && tile < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
-                next = page_of(i16 + 1);
-                oks_before = oks;
-                oks = __ballot_sync(0xffffffffu, ok);
-                const uint32_t in_page = tile - quot(tile) * page_tiles;
-                src = a.data + ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + in_page) * TILE;
-            }
-            if (lane >> 1 == (issued & 15)) {  // each lane of the two: its tile, or none
-                const bool ok = !dead && (oks >> lane & 1u);
-                mbar_arrive_expect_tx(&bars[wid][stage], ok ? TILE : 0);
-                if (ok) bulk_load(ring + stage * S::STAGE + (lane & 1) * TILE, src, TILE, &bars[wid][stage]);
-            }
-            issued++;
-        };
-        while (issued < STAGES - 1 && issued < n_units) fetch(issued);
 
         // Weights are 2^(x - ref).  With vexp the exponent of the largest
         // value scale so far (below 2^(vexp - 14)), a weight times a scale
@@ -639,7 +668,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
             }
         __syncthreads();
         const bool whole = ua == 0 && ub == s.units;
-        float *part = a.work + (2 * static_cast<int64_t>(blockIdx.x) + (at == cut.at ? 0 : 1)) * part_floats(RB, D);
+        float *part = a.work + NOTE_FLOATS * gridDim.x + (2 * static_cast<int64_t>(blockIdx.x) + (at == cut.at ? 0 : 1)) * part_floats(RB, D);
         for (int k = threadIdx.x; k < RB * (D / 4); k += WARPS * 32) {
             const int row = k / (D / 4), c = k % (D / 4) * 4, r = row0 + row;
             if (r >= s.count * a.share) continue;
@@ -667,7 +696,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                 continue;
             }
             if (a.one) sum += exp2_fast(-off);
-            finish<T, D>(a, s, head, r, c, o, top, sum);
+            finish<T, D>(a, s.first, head, r, c, o, top, sum);
         }
         fence_proxy_async_smem();  // the rings' next writers are bulk copies
         __syncthreads();
@@ -675,72 +704,56 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
     }
 }
 
-// Joins the pieces of the item that the start of part i + 1 cuts, for the
-// first such cut in the item.  Each thread adds up four channels of one row
-// over every SETS-th piece, eight loads in flight; the sets are then added in
-// order, so the result does not depend on timing.
+// Joins an item's pieces, found by the notes that the parts left: block i
+// looks at note i.  A warp adds up one row over every SETS-th piece, four
+// channels a lane, sixteen loads in flight; the sets are then added in order,
+// so the result does not depend on timing.
 constexpr int JOIN = 512;
 template <typename T, int D, int RB>
-__global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a, int64_t grid) {
-    constexpr int VALS = RB * D / 4, SETS = JOIN / VALS;
-    __shared__ int64_t scan[2 * (JOIN / 32) + 2];
-    __shared__ float4 sums[SETS][VALS];
+__global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a) {
+    constexpr int LANES = D / 4, SETS = JOIN / (RB * LANES), DEPTH = 16;
+    __shared__ float4 sums[SETS][RB * LANES];
     __shared__ float tops[SETS][RB], weights[SETS][RB];
     grid_dep_wait();
-    const int64_t i = blockIdx.x + 1;
-    const Cut c = cut_for<RB, JOIN / 32>(a, i, grid, scan);
-    if (i >= c.n) return;
-    const Seq s = seq_of<RB>(a, c.b);
-    const int item = static_cast<int>((c.at - c.base) / s.units);
-    const int64_t start = c.base + static_cast<int64_t>(item) * s.units, end = start + s.units;
-    const int64_t before = c.total * (i - 1) / c.n;
-    if (start == c.at || before > start) return;
-    int64_t last = i;  // pieces: the last one of part i - 1, then the first ones of parts i .. last
-    {
-        // part j starts before `end`: total j / n < end
-        last = (end * c.n + c.total - 1) / c.total - 1;
-        while (last + 1 < c.n && c.total * (last + 1) / c.n < end) last++;
-        while (last > i && c.total * last / c.n >= end) last--;
-    }
-    const int pieces = static_cast<int>(last - i + 2);
-    const int64_t first = 2 * (i - 1) + (before == start ? 0 : 1);
-    const int head = item / s.blocks, row0 = item % s.blocks * RB;
-    const int set = threadIdx.x / VALS, row = threadIdx.x % VALS / (D / 4), ch = threadIdx.x % (D / 4) * 4;
+    const Note note = reinterpret_cast<const Note *>(a.work)[blockIdx.x];
+    if (note.pieces == 0) return;
+    const float *parts = a.work + NOTE_FLOATS * gridDim.x;
+    const int at = threadIdx.x % (RB * LANES), set = threadIdx.x / (RB * LANES), row = at / LANES, ch = at % LANES * 4;
     float top = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p0 = set; p0 < pieces; p0 += 8 * SETS) {
-        float pm[8], pl[8];
-        float4 v[8];
+    for (int p0 = set; p0 < note.pieces; p0 += DEPTH * SETS) {
+        float pm[DEPTH], pl[DEPTH];
+        float4 v[DEPTH];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < DEPTH; k++) {
             const int p = p0 + k * SETS;
-            const float *src = a.work + (p == 0 ? first : 2 * (i + p - 1)) * part_floats(RB, D);
-            pm[k] = p < pieces ? src[RB * D + row] : -INFINITY;
-            pl[k] = p < pieces ? src[RB * D + RB + row] : 0.0f;
-            v[k] = p < pieces ? *reinterpret_cast<const float4 *>(src + row * D + ch) : make_float4(0, 0, 0, 0);
+            const float *src = parts + (p == 0 ? note.slot : 2 * (blockIdx.x + static_cast<int64_t>(p) - 1)) * part_floats(RB, D);
+            pm[k] = p < note.pieces ? src[RB * D + row] : -INFINITY;
+            pl[k] = p < note.pieces ? src[RB * D + RB + row] : 0.0f;
+            v[k] = p < note.pieces ? *reinterpret_cast<const float4 *>(src + row * D + ch) : make_float4(0, 0, 0, 0);
         }
         float now = top;
 #pragma unroll
-        for (int k = 0; k < 8; k++) now = fmaxf(now, pm[k]);
+        for (int k = 0; k < DEPTH; k++) now = fmaxf(now, pm[k]);
         const float off = now == -INFINITY ? 0.0f : now, f = exp2_fast(top - off);
         top = now;
         sum *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < DEPTH; k++) {
             const float w = exp2_fast(pm[k] - off);
             sum = fmaf(pl[k], w, sum);
             o.x = fmaf(v[k].x, w, o.x), o.y = fmaf(v[k].y, w, o.y);
             o.z = fmaf(v[k].z, w, o.z), o.w = fmaf(v[k].w, w, o.w);
         }
     }
-    sums[set][threadIdx.x % VALS] = o;
+    sums[set][at] = o;
     if (ch == 0) {
         tops[set][row] = top;
         weights[set][row] = sum;
     }
     __syncthreads();
-    const int r = row0 + row;
-    if (set > 0 || r >= s.count * a.share) return;
+    const int r = note.row0 + row;
+    if (set > 0 || r >= note.rows) return;
     top = a.one ? 0.0f : -INFINITY;
 #pragma unroll
     for (int k = 0; k < SETS; k++) top = fmaxf(top, tops[k][row]);
@@ -750,11 +763,11 @@ __global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a, int64_
 #pragma unroll
     for (int k = 0; k < SETS; k++) {
         const float w = exp2_fast(tops[k][row] - off);
-        const float4 v = sums[k][threadIdx.x];
+        const float4 v = sums[k][at];
         sum = fmaf(weights[k][row], w, sum);
         o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
     }
-    finish<T, D>(a, s, head, r, ch, o, top, sum);
+    finish<T, D>(a, note.first, note.head, r, ch, o, top, sum);
 }
 
 // Eight columns (one group of 8 rows) unless a kv head has more rows than that.
@@ -769,6 +782,10 @@ int64_t grid_of(const st_handle *h, int64_t batch, int64_t rows, int64_t max_q, 
     return static_cast<int64_t>(std::max(1.0, std::min(static_cast<double>(most), units / MIN_UNITS + 1)));
 }
 
+int64_t work_bytes(int64_t grid, int nt, int d) {
+    return grid * static_cast<int64_t>(sizeof(Note)) + 2 * grid * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
+}
+
 template <typename T, int D, int G, int NT>
 st_status launch(st_handle *h, const AttnArgs &a) {
     using S = Shape<T, D, G, NT>;
@@ -777,8 +794,8 @@ st_status launch(st_handle *h, const AttnArgs &a) {
     ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn<T, D, G, NT>, dim3(static_cast<unsigned>(grid)),
                                          dim3(WARPS * 32), S::SMEM, a));
     if (st_status s = st_after_launch(h, "k_kv4_attn"); s != ST_OK || grid == 1) return s;
-    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_join<T, D, S::RB>, dim3(static_cast<unsigned>(grid - 1)),
-                                         dim3(JOIN), 0, a, grid));
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_join<T, D, S::RB>, dim3(static_cast<unsigned>(grid)),
+                                         dim3(JOIN), 0, a));
     return st_after_launch(h, "k_kv4_attn_join");
 }
 
@@ -797,7 +814,7 @@ extern "C" st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t 
         return h->fail(ST_INVALID_ARG, "st_kv4_attn_workspace: bad arguments");
     const int nt = columns_of(max_q, heads / kv_heads);
     const int64_t grid = grid_of(h, batch, rows, max_q, kv_heads, heads / kv_heads, nt, 1ll << 30, nt == 1 ? 4 : 2);
-    *bytes = 2 * grid * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
+    *bytes = work_bytes(grid, nt, d);
     return ST_OK;
 }
 
@@ -824,7 +841,7 @@ extern "C" st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, i
     if (!q_start) max_q = 1;
     const int share = heads / kv_heads, nt = columns_of(max_q, share);
     const int64_t grid = grid_of(h, batch, rows, max_q, kv_heads, share, nt, max_pages * page, nt == 1 ? 4 : 2);
-    const int64_t need = 2 * grid * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
+    const int64_t need = work_bytes(grid, nt, d);
     if (workspace) {
         if (workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
             return h->fail(ST_INVALID_ARG, "st_kv4_attn: the workspace needs %lld aligned bytes",
