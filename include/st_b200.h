@@ -416,9 +416,9 @@ ST_API st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, int64
                              const int32_t *kv_len, const int32_t *q_start, int64_t batch, int64_t rows,
                              int64_t max_q, float scale, int32_t causal, int32_t one, int32_t window, int32_t dtype,
                              void *workspace, int64_t workspace_bytes);
-/* Bytes of the workspace for calls of these shapes. */
-ST_API st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int32_t heads,
-                                       int32_t kv_heads, int32_t d, int64_t *bytes);
+/* Bytes of the workspace for calls of these shapes; max_keys: max_pages * page. */
+ST_API st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int64_t max_keys,
+                                       int32_t heads, int32_t kv_heads, int32_t d, int64_t *bytes);
 /* out [rows, vocab] (rows out_ld apart; may be logits itself) = logits (rows
  * ld apart) after, in f32 and in this order: repetition, x / repetition[r] (x >
  * 0) or x * repetition[r] for tokens in the row's history; - frequency[r] *

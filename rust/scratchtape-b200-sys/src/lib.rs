@@ -195,8 +195,8 @@ extern "C" {
         group: i32, pages: *const i32, max_pages: i64, kv_len: *const i32, q_start: *const i32, batch: i64,
         rows: i64, max_q: i64, scale: f32, causal: i32, one: i32, window: i32, dtype: i32,
         workspace: *mut c_void, workspace_bytes: i64) -> st_status;
-    pub fn st_kv4_attn_workspace(h: *mut st_handle, batch: i64, rows: i64, max_q: i64, heads: i32,
-        kv_heads: i32, d: i32, bytes: *mut i64) -> st_status;
+    pub fn st_kv4_attn_workspace(h: *mut st_handle, batch: i64, rows: i64, max_q: i64, max_keys: i64,
+        heads: i32, kv_heads: i32, d: i32, bytes: *mut i64) -> st_status;
     pub fn st_logits_adjust(h: *mut st_handle, logits: *const c_void, ld: i64, out: *mut c_void, out_ld: i64,
         rows: i64, vocab: i64, tokens: *const i32, starts: *const i32, prompt: *const i32,
         repetition: *const f32, presence: *const f32, frequency: *const f32, bias_tokens: *const i32,

@@ -40,7 +40,10 @@ struct AttnArgs {
     float scale_log2;  // scale * log2(e): scores are kept in units of log 2
     int causal, one, window;
     int vec;           // rows of q start on 16-byte boundaries
-    float *work;       // pieces' partial results
+    int sms, parts;    // parts at most
+    int item_blocks;   // blocks of rows of a sequence at most, where notes go by item; else 0
+    int64_t notes;     // notes at the start of the workspace
+    float *work;       // notes, then the pieces' partial results
     int *status;
 };
 
@@ -48,7 +51,7 @@ struct AttnArgs {
 
 constexpr int UNIT = 32;     // keys of one step of a warp: two tiles
 constexpr int WARPS = 4;     // warps of a block; they take a piece's units in turn
-constexpr int MIN_UNITS = 4;  // units a block takes at least (one for each warp)
+constexpr int MIN_UNITS = 4;  // units of a part at least (one for each warp)
 
 struct Seq {
     int64_t first;         // its first row
@@ -103,67 +106,73 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
 }
 
+// The units of all items (an item: a kv head's block of rows), one after the
+// other, are cut into n equal parts, one for each team of WARPS warps; part i
+// is that of team i / SMs of block i % SMs.  Teams of one block advance evenly.
+// Separate blocks on an SM do not (the SM issues for the oldest first): four
+// with equal parts ended after 162, 176, 196 and 217 us, the last ones alone.
 struct Cut {
-    int64_t total;  // units of all items (an item: a kv head's block of rows)
-    int64_t n;      // blocks that get some
-    int64_t each, more;   // `each` units, the first `more` blocks one more
-    int64_t at, b, base;  // where this one's part starts, in which sequence, and where that starts
-    __device__ int64_t start(int64_t i) const { return each * i + min(i, more); }
+    int64_t total, each;
+    int n, more;  // `each` units, the first `more` parts one more
+    __device__ void divide(int64_t units, int parts) {
+        total = units;
+        n = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(parts), total / MIN_UNITS)));
+        each = quotient(total, n);
+        more = static_cast<int>(total - each * n);
+    }
+    __device__ int64_t start(int64_t i) const { return each * i + min(i, static_cast<int64_t>(more)); }
+    __device__ int64_t part_of(int64_t unit) const {
+        const int64_t wide = more * (each + 1);
+        return unit < wide ? quotient(unit, each + 1) : more + quotient(unit - wide, each);
+    }
 };
 
-// Units [start(i), start(i + 1)) are block i's.  Every thread of the
-// block calls it; smem holds 2 * WARPS + 2 int64.
-template <int RB>
-__device__ Cut cut_for(const AttnArgs &a, int64_t i, int64_t grid, int64_t *smem) {
-    const int lane = threadIdx.x & 31, wid = threadIdx.x / 32;
-    Cut c;
-    int64_t mine = 0, v = 0;
-    for (int64_t b = threadIdx.x; b < a.batch; b += blockDim.x) mine += v = weight_of<RB>(a, b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) smem[wid] = mine;
-    __syncthreads();
-    c.total = 0;
-    for (int w = 0; w < WARPS; w++) c.total += smem[w];
-    c.n = max(static_cast<int64_t>(1), min(grid, c.total / MIN_UNITS));
-    c.each = quotient(c.total, c.n);
-    c.more = c.total - c.each * c.n;
-    c.at = c.start(i);
-    int64_t carry = 0;
-    for (int64_t b0 = 0; b0 < a.batch; b0 += blockDim.x) {
-        const int64_t b = b0 + threadIdx.x;
-        if (a.batch > blockDim.x) v = b < a.batch ? weight_of<RB>(a, b) : 0;
-        int64_t incl = b < a.batch ? v : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += t;
-        }
-        if (lane == 31) smem[WARPS + wid] = incl;
-        __syncthreads();
-        int64_t before = carry;
-        for (int w = 0; w < WARPS; w++) {
-            if (w < wid) before += smem[WARPS + w];
-            carry += smem[WARPS + w];
-        }
-        const int64_t end = before + incl, start = end - v;
-        if (b < a.batch && start <= c.at && c.at < end) {
-            smem[2 * WARPS] = b;
-            smem[2 * WARPS + 1] = start;
-        }
-        __syncthreads();
-    }
-    c.b = smem[2 * WARPS];
-    c.base = smem[2 * WARPS + 1];
-    return c;
+__device__ __forceinline__ int team_thread() { return threadIdx.x % (32 * WARPS); }
+// A barrier for the team's warps.
+__device__ __forceinline__ void team_sync() {
+    asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.x / (32 * WARPS) + 1), "n"(32 * WARPS) : "memory");
 }
 
-// What a part leaves for the join, at the start of the workspace: the item
-// that its start cuts, if it is the first part to cut it.
+// Where each of 32 * WARPS runs of sequences starts among the units, and the
+// end: starts[0 .. 32 * WARPS].  Every thread of the team calls it.
+template <int RB>
+__device__ void sum_units(const AttnArgs &a, int64_t *starts, int64_t *scratch) {
+    const int lane = threadIdx.x & 31, wid = team_thread() / 32;
+    const int64_t run = (a.batch + 32 * WARPS - 1) / (32 * WARPS);
+    int64_t incl = 0;
+    for (int64_t b = team_thread() * run; b < min(a.batch, (team_thread() + 1) * run); b++) incl += weight_of<RB>(a, b);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) scratch[wid] = incl;
+    team_sync();
+    for (int w = 0; w < wid; w++) incl += scratch[w];
+    starts[team_thread() + 1] = incl;
+    if (team_thread() == 0) starts[0] = 0;
+    team_sync();
+}
+
+// The sequence that unit `at` belongs to, or the first of its run: the caller
+// goes on from there.
+__device__ __forceinline__ int64_t run_of(const AttnArgs &a, const int64_t *starts, int64_t at, int64_t &base) {
+    int i = 0;
+#pragma unroll
+    for (int step = 16 * WARPS; step > 0; step >>= 1)
+        if (starts[i + step] <= at) i += step;
+    base = starts[i];
+    return i * ((a.batch + 32 * WARPS - 1) / (32 * WARPS));
+}
+
+// What the parts leave for the join, at the start of the workspace: by item
+// (its pieces, 0 if it is whole) where the items are few, else by part (the
+// item that its start cuts, if it is the first part to cut it).
 struct Note {
-    int pieces;  // of that item: in `slot`, then the first ones of this part and those after it (0: none)
+    int pieces;  // in `slot`, then the first ones of part `part` and those after it
     int head, row0, rows;  // rows: of the sequence, times the shared heads
-    int64_t first, slot;
+    int64_t first, slot, part;
+    int64_t unused;
 };
 constexpr int NOTE_FLOATS = sizeof(Note) / 4;
 
@@ -250,6 +259,8 @@ __device__ __forceinline__ void load8(const T *p, int vec, float (&x)[8]) {
 
 // ---- the kernel ---------------------------------------------------------------
 
+constexpr int MOST_TEAMS = 4;  // teams that an SM holds at most
+
 template <typename T, int D, int G, int NT>
 struct Shape {
     static constexpr bool F32 = std::is_same<T, float>::value;
@@ -258,7 +269,7 @@ struct Shape {
     static constexpr int RING = STAGES * STAGE;  // bytes of a warp's ring; holds its [RB][D + 2] floats at the end
     static_assert(RING >= RB * (D + 2) * 4, "a warp's result fits its ring");
     static constexpr int SMEM = WARPS * RING;
-    static constexpr int PER_SM = NT == 1 ? (SMEM <= 56000 ? 4 : 3) : 2;  // blocks that an SM holds
+    static constexpr int TEAMS = NT == 1 ? (SMEM <= 56000 ? MOST_TEAMS : 3) : 2;  // of a block, one block an SM
 };
 
 // Writes four channels of row r's result and, once, its log-sum-exp.
@@ -273,36 +284,45 @@ __device__ __forceinline__ void finish(const AttnArgs &a, int64_t first, int hea
     if (a.lse && c == 0) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
 }
 
-// One block: its part of the units, piece by piece (a piece: consecutive
+// One team of WARPS warps: its part of the units, piece by piece (a piece: consecutive
 // units of one item).  Each warp has a ring of STAGES steps of two tiles that
 // bulk copies fill, and a running maximum, sum and result of its own; the
-// warps' results are joined at the end of a piece.  An item that one block
+// warps' results are joined at the end of a piece.  An item that one team
 // holds whole is written out; parts of one go to the workspace and are joined
 // by k_kv4_attn_join, which finds them by the notes that the parts leave.
 template <typename T, int D, int G, int NT>
-__global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_attn(const AttnArgs a) {
+__global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_kv4_attn(const AttnArgs a) {
     using S = Shape<T, D, G, NT>;
     constexpr int NG = S::NG, RB = S::RB, TILE = S::TILE, STAGES = S::STAGES, KS = G / 16, MT = D / 16;
     constexpr int W = G / 32;          // words of a thread in a group's row of key codes
     constexpr int QS = S::F32 ? 2 : 1;  // f32: queries and weights as two f16 terms, 22 bits
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bars[WARPS][STAGES];
-    __shared__ int64_t scan[2 * WARPS + 2];
-    const int lane = threadIdx.x & 31, wid = threadIdx.x / 32, g = lane >> 2, t = lane & 3;
+    extern __shared__ __align__(128) uint8_t all_smem[];
+    __shared__ uint64_t all_bars[S::TEAMS][WARPS][STAGES];
+    __shared__ Cut cuts[S::TEAMS];
+    __shared__ int64_t all_starts[S::TEAMS][32 * WARPS + 1], all_scratch[S::TEAMS][WARPS];
+    const int team = threadIdx.x / (32 * WARPS), tid = team_thread();
+    const int lane = tid & 31, wid = tid / 32, g = lane >> 2, t = lane & 3;
+    uint8_t *smem = all_smem + team * S::SMEM;
+    uint64_t(*bars)[STAGES] = all_bars[team];
+    int64_t *starts = all_starts[team];
     uint8_t *ring = smem + wid * S::RING;
     if (lane == 0)
         for (int i = 0; i < STAGES; i++) mbar_init(&bars[wid][i], 2);
     fence_mbar_init();
     grid_dep_wait();
-    const Cut cut = cut_for<RB>(a, blockIdx.x, gridDim.x, scan);
+    sum_units<RB>(a, starts, all_scratch[team]);
+    Cut &cut = cuts[team];
+    if (tid == 0) cut.divide(starts[32 * WARPS], a.parts);
+    team_sync();
+    const int64_t part = blockIdx.x + static_cast<int64_t>(team) * a.sms;
     grid_dep_launch();
-    Note *note = reinterpret_cast<Note *>(a.work) + blockIdx.x;
-    if (threadIdx.x == 0) note->pieces = 0;
-    if (blockIdx.x >= cut.n) return;
-    const int64_t until = cut.start(blockIdx.x + 1);
-    int64_t at = cut.at, b = cut.b, base = cut.base;
+    Note *notes = reinterpret_cast<Note *>(a.work);
+    if (tid == 0 && a.item_blocks == 0 && part < a.parts) notes[part].pieces = 0;
+    if (part >= cut.n) return;
     uint32_t phases = 0;  // bit i: the parity that stage i's next step completes
     bool dead = false;
+    const int64_t from = cut.start(part), until = cut.start(part + 1);
+    int64_t at = from, base, b = run_of(a, starts, at, base);
     while (at < until) {
         Seq s = seq_of<RB>(a, b);
         for (int64_t w; at >= base + (w = static_cast<int64_t>(s.units) * s.blocks * a.kv_heads);) {
@@ -313,13 +333,15 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
         const int ua = static_cast<int>(at - base - static_cast<int64_t>(item) * s.units);
         const int ub = static_cast<int>(min(static_cast<int64_t>(s.units), ua + (until - at)));
         const int head = item / s.blocks, row0 = item % s.blocks * RB;
-        if (at == cut.at && ua > 0 && threadIdx.x == 0) {
-            const int64_t start = at - ua, before = cut.start(blockIdx.x - 1);
-            int64_t last = blockIdx.x;
-            while (last + 1 < cut.n && cut.start(last + 1) < start + s.units) last++;
-            if (before <= start)
-                *note = Note{static_cast<int>(last - blockIdx.x) + 2, head, row0, s.count * a.share, s.first,
-                             2 * (static_cast<int64_t>(blockIdx.x) - 1) + (before == start ? 0 : 1)};
+        if (tid == 0) {
+            Note &note = notes[a.item_blocks ? b * a.item_blocks * a.kv_heads + item : part];
+            const int64_t start = at - ua, before = part > 0 ? cut.start(part - 1) : 0;
+            if (at == from && ua > 0 && before <= start) {
+                note = Note{static_cast<int>(cut.part_of(start + s.units - 1) - part) + 2, head, row0, s.count * a.share,
+                            s.first, 2 * (part - 1) + (before == start ? 0 : 1), part, 0};
+            } else if (a.item_blocks && ua == 0 && ub == s.units) {
+                note.pieces = 0;
+            }
         }
 
         // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 2j and
@@ -666,10 +688,10 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                     mine[RB * D + RB + row] = ls;
                 }
             }
-        __syncthreads();
+        team_sync();
         const bool whole = ua == 0 && ub == s.units;
-        float *part = a.work + NOTE_FLOATS * gridDim.x + (2 * static_cast<int64_t>(blockIdx.x) + (at == cut.at ? 0 : 1)) * part_floats(RB, D);
-        for (int k = threadIdx.x; k < RB * (D / 4); k += WARPS * 32) {
+        float *piece = a.work + NOTE_FLOATS * a.notes + (2 * part + (at == from ? 0 : 1)) * part_floats(RB, D);
+        for (int k = tid; k < RB * (D / 4); k += WARPS * 32) {
             const int row = k / (D / 4), c = k % (D / 4) * 4, r = row0 + row;
             if (r >= s.count * a.share) continue;
             float wm[WARPS], top = -INFINITY, sum = 0.0f;
@@ -688,10 +710,10 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
                 o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
             }
             if (!whole) {
-                *reinterpret_cast<float4 *>(part + row * D + c) = o;
+                *reinterpret_cast<float4 *>(piece + row * D + c) = o;
                 if (c == 0) {
-                    part[RB * D + row] = top;
-                    part[RB * D + RB + row] = sum;
+                    piece[RB * D + row] = top;
+                    piece[RB * D + RB + row] = sum;
                 }
                 continue;
             }
@@ -699,26 +721,31 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<T, D, G, NT>::PER_SM) k_kv4_
             finish<T, D>(a, s.first, head, r, c, o, top, sum);
         }
         fence_proxy_async_smem();  // the rings' next writers are bulk copies
-        __syncthreads();
+        team_sync();
         at += ub - ua;
     }
 }
 
-// Joins an item's pieces, found by the notes that the parts left: block i
-// looks at note i.  A warp adds up one row over every SETS-th piece, four
-// channels a lane, sixteen loads in flight; the sets are then added in order,
-// so the result does not depend on timing.
+// Joins an item's pieces, found by the notes that the parts left: block x
+// looks at note x, and takes its rows ROWS blockIdx.y ....  A row is added up
+// over every SETS-th piece, four channels a thread, sixteen loads in flight;
+// the sets are then added in order, so the result does not depend on timing.
 constexpr int JOIN = 512;
-template <typename T, int D, int RB>
+template <typename T, int D, int RB, int ROWS>
 __global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a) {
-    constexpr int LANES = D / 4, SETS = JOIN / (RB * LANES), DEPTH = 16;
-    __shared__ float4 sums[SETS][RB * LANES];
-    __shared__ float tops[SETS][RB], weights[SETS][RB];
+    constexpr int LANES = D / 4, SETS = JOIN / (ROWS * LANES), DEPTH = 16;
+    __shared__ float4 sums[SETS][ROWS * LANES];
+    __shared__ float tops[SETS][ROWS], weights[SETS][ROWS];
     grid_dep_wait();
+    if (a.item_blocks) {
+        const int per = a.item_blocks * a.kv_heads, b = blockIdx.x / per;
+        if (blockIdx.x - b * per >= seq_of<RB>(a, b).blocks * a.kv_heads) return;
+    }
     const Note note = reinterpret_cast<const Note *>(a.work)[blockIdx.x];
     if (note.pieces == 0) return;
-    const float *parts = a.work + NOTE_FLOATS * gridDim.x;
-    const int at = threadIdx.x % (RB * LANES), set = threadIdx.x / (RB * LANES), row = at / LANES, ch = at % LANES * 4;
+    const float *parts = a.work + NOTE_FLOATS * a.notes;
+    const int at = threadIdx.x % (ROWS * LANES), set = threadIdx.x / (ROWS * LANES), mine = at / LANES;
+    const int row = blockIdx.y * ROWS + mine, ch = at % LANES * 4;
     float top = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p0 = set; p0 < note.pieces; p0 += DEPTH * SETS) {
@@ -727,7 +754,7 @@ __global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < DEPTH; k++) {
             const int p = p0 + k * SETS;
-            const float *src = parts + (p == 0 ? note.slot : 2 * (blockIdx.x + static_cast<int64_t>(p) - 1)) * part_floats(RB, D);
+            const float *src = parts + (p == 0 ? note.slot : 2 * (note.part + p - 1)) * part_floats(RB, D);
             pm[k] = p < note.pieces ? src[RB * D + row] : -INFINITY;
             pl[k] = p < note.pieces ? src[RB * D + RB + row] : 0.0f;
             v[k] = p < note.pieces ? *reinterpret_cast<const float4 *>(src + row * D + ch) : make_float4(0, 0, 0, 0);
@@ -748,23 +775,23 @@ __global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a) {
     }
     sums[set][at] = o;
     if (ch == 0) {
-        tops[set][row] = top;
-        weights[set][row] = sum;
+        tops[set][mine] = top;
+        weights[set][mine] = sum;
     }
     __syncthreads();
     const int r = note.row0 + row;
     if (set > 0 || r >= note.rows) return;
     top = a.one ? 0.0f : -INFINITY;
 #pragma unroll
-    for (int k = 0; k < SETS; k++) top = fmaxf(top, tops[k][row]);
+    for (int k = 0; k < SETS; k++) top = fmaxf(top, tops[k][mine]);
     const float off = top == -INFINITY ? 0.0f : top;
     sum = a.one ? exp2_fast(-off) : 0.0f;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < SETS; k++) {
-        const float w = exp2_fast(tops[k][row] - off);
+        const float w = exp2_fast(tops[k][mine] - off);
         const float4 v = sums[k][at];
-        sum = fmaf(weights[k][row], w, sum);
+        sum = fmaf(weights[k][mine], w, sum);
         o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
     }
     finish<T, D>(a, note.first, note.head, r, ch, o, top, sum);
@@ -773,29 +800,47 @@ __global__ void __launch_bounds__(JOIN) k_kv4_attn_join(const AttnArgs a) {
 // Eight columns (one group of 8 rows) unless a kv head has more rows than that.
 int columns_of(int64_t max_q, int share) { return max_q * share > 8 ? 2 : 1; }
 
-int64_t grid_of(const st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int kv_heads, int share, int nt,
-                int64_t max_keys, int per_sm) {
-    const int rb = 8 * nt;
-    const int64_t blocks = std::min((max_q * share + rb - 1) / rb * batch, (rows * share + rb - 1) / rb + batch);
-    const double units = static_cast<double>(blocks) * kv_heads * static_cast<double>((max_keys + UNIT - 1) / UNIT + 1);
-    const int64_t most = static_cast<int64_t>(h->num_sms) * per_sm;
-    return static_cast<int64_t>(std::max(1.0, std::min(static_cast<double>(most), units / MIN_UNITS + 1)));
-}
-
-int64_t work_bytes(int64_t grid, int nt, int d) {
-    return grid * static_cast<int64_t>(sizeof(Note)) + 2 * grid * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
-}
+// How a call is laid out, from what the host knows of it.
+struct Plan {
+    int64_t parts, notes;
+    int item_blocks;
+    bool deep;            // many pieces of few items: the join's rows go to several blocks
+    Plan(const st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int kv_heads, int share, int nt,
+         int64_t max_keys, int teams) {
+        const int rb = 8 * nt;
+        const int at_once = h->num_sms * teams;
+        const int64_t per_seq = (max_q * share + rb - 1) / rb;
+        const int64_t blocks = std::min(per_seq * batch, (rows * share + rb - 1) / rb + batch);
+        const double units = static_cast<double>(blocks) * kv_heads * static_cast<double>((max_keys + UNIT - 1) / UNIT + 1);
+        parts = static_cast<int64_t>(std::max(1.0, std::min(1.0 * at_once, units / MIN_UNITS + 1)));
+        const bool by_item = per_seq * batch <= at_once / kv_heads;
+        item_blocks = by_item ? static_cast<int>(per_seq) : 0;
+        notes = by_item ? per_seq * batch * kv_heads : parts;
+        deep = by_item && parts >= 16 * notes;
+    }
+    int64_t bytes(int nt, int d) const {
+        return std::max(notes, parts) * static_cast<int64_t>(sizeof(Note)) + 2 * parts * part_floats(8 * nt, d) * static_cast<int64_t>(sizeof(float));
+    }
+};
 
 template <typename T, int D, int G, int NT>
-st_status launch(st_handle *h, const AttnArgs &a) {
+st_status launch(st_handle *h, AttnArgs a) {
     using S = Shape<T, D, G, NT>;
-    const int64_t grid = grid_of(h, a.batch, a.rows, a.max_q, a.kv_heads, a.share, NT, a.max_pages * a.page, S::PER_SM);
-    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_kv4_attn<T, D, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn<T, D, G, NT>, dim3(static_cast<unsigned>(grid)),
-                                         dim3(WARPS * 32), S::SMEM, a));
-    if (st_status s = st_after_launch(h, "k_kv4_attn"); s != ST_OK || grid == 1) return s;
-    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_join<T, D, S::RB>, dim3(static_cast<unsigned>(grid)),
-                                         dim3(JOIN), 0, a));
+    const Plan plan(h, a.batch, a.rows, a.max_q, a.kv_heads, a.share, NT, a.max_pages * a.page, S::TEAMS);
+    a.sms = h->num_sms;
+    a.parts = static_cast<int>(plan.parts);
+    a.item_blocks = plan.item_blocks;
+    a.notes = plan.notes;
+    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_kv4_attn<T, D, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          S::TEAMS * S::SMEM));
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn<T, D, G, NT>, dim3(static_cast<unsigned>(std::min<int64_t>(plan.parts, h->num_sms))),
+                                         dim3(S::TEAMS * WARPS * 32), S::TEAMS * S::SMEM, a));
+    if (st_status s = st_after_launch(h, "k_kv4_attn"); s != ST_OK || plan.parts == 1) return s;
+    const dim3 notes(static_cast<unsigned>(plan.notes), plan.deep ? S::RB / 2 : 1);
+    if (plan.deep)
+        ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_join<T, D, S::RB, 2>, notes, dim3(JOIN), 0, a));
+    else
+        ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_join<T, D, S::RB, S::RB>, notes, dim3(JOIN), 0, a));
     return st_after_launch(h, "k_kv4_attn_join");
 }
 
@@ -806,15 +851,14 @@ st_status by_columns(st_handle *h, const AttnArgs &a, int nt) {
 
 }  // namespace
 
-extern "C" st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int32_t heads,
-                                           int32_t kv_heads, int32_t d, int64_t *bytes) {
+extern "C" st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows, int64_t max_q, int64_t max_keys,
+                                           int32_t heads, int32_t kv_heads, int32_t d, int64_t *bytes) {
     if (!h) return ST_INVALID_ARG;
     if (!bytes || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || batch < 0 || rows < 0 || max_q < 0 ||
-        (d != 64 && d != 128))
+        max_keys < 0 || (d != 64 && d != 128))
         return h->fail(ST_INVALID_ARG, "st_kv4_attn_workspace: bad arguments");
     const int nt = columns_of(max_q, heads / kv_heads);
-    const int64_t grid = grid_of(h, batch, rows, max_q, kv_heads, heads / kv_heads, nt, 1ll << 30, nt == 1 ? 4 : 2);
-    *bytes = work_bytes(grid, nt, d);
+    *bytes = Plan(h, batch, rows, max_q, kv_heads, heads / kv_heads, nt, max_keys, MOST_TEAMS).bytes(nt, d);
     return ST_OK;
 }
 
@@ -840,8 +884,7 @@ extern "C" st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, i
     cudaSetDevice(h->device);
     if (!q_start) max_q = 1;
     const int share = heads / kv_heads, nt = columns_of(max_q, share);
-    const int64_t grid = grid_of(h, batch, rows, max_q, kv_heads, share, nt, max_pages * page, nt == 1 ? 4 : 2);
-    const int64_t need = work_bytes(grid, nt, d);
+    const int64_t need = Plan(h, batch, rows, max_q, kv_heads, share, nt, max_pages * page, MOST_TEAMS).bytes(nt, d);
     if (workspace) {
         if (workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
             return h->fail(ST_INVALID_ARG, "st_kv4_attn: the workspace needs %lld aligned bytes",
@@ -854,7 +897,7 @@ extern "C" st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, i
     const AttnArgs a = {q, q_token, q_head, o, lse, static_cast<const uint8_t *>(data), n_pages, page, heads,
                         kv_heads, share, pages, max_pages, kv_len, q_start, batch, rows, static_cast<int>(max_q),
                         page == 16 ? 0u : static_cast<uint32_t>(((1ull << 32) + page / 16 - 1) / (page / 16)),
-                        scale * 1.44269504088896341f, causal, one, window, vec, static_cast<float *>(workspace),
+                        scale * 1.44269504088896341f, causal, one, window, vec, 0, 0, 0, 0, static_cast<float *>(workspace),
                         h->d_status};
 #define KV4_CASE(D_, G_)                                                               \
     if (d == D_ && group == G_) {                                                      \

@@ -146,7 +146,7 @@ def attend(q: torch.Tensor, data: torch.Tensor, pages: torch.Tensor, kv_len: tor
     if rows and batch:
         h = handle(data.device)
         need = ctypes.c_int64()
-        h.call("st_kv4_attn_workspace", batch, rows, max_q, heads, kv_heads, d, ctypes.byref(need))
+        h.call("st_kv4_attn_workspace", batch, rows, max_q, pages.shape[1] * page, heads, kv_heads, d, ctypes.byref(need))
         # torch's allocator gives each stream, and each captured graph, a workspace of its own
         work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
         h.call("st_kv4_attn", ptr(q), q.stride(0), q.stride(1), ptr(o), ptr(lse), ptr(data), n_pages, page, heads,
