@@ -101,8 +101,10 @@ __device__ __forceinline__ int64_t weight_of(const AttnArgs &a, int64_t b) {
     return static_cast<int64_t>(s.units) * s.blocks * a.kv_heads;
 }
 
-// a / b; 64-bit division only where it is needed (it costs about 100 instructions).
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+// a / b; 64-bit division, about 100 instructions, only where it is needed.  Not
+// inlined: the kernels start with cold instruction caches, and what their first
+// microseconds run is kept short.
+__device__ __noinline__ int64_t quotient(int64_t a, int64_t b) {
     return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
 }
 
@@ -299,6 +301,8 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
     extern __shared__ __align__(128) uint8_t all_smem[];
     __shared__ uint64_t all_bars[S::TEAMS][WARPS][STAGES];
     __shared__ Cut cuts[S::TEAMS];
+    __shared__ float q_sums[S::TEAMS][RB][NG];
+    __shared__ uint32_t q_tops[S::TEAMS][WARPS];
     __shared__ int64_t all_starts[S::TEAMS][32 * WARPS + 1], all_scratch[S::TEAMS][WARPS];
     const int team = threadIdx.x / (32 * WARPS), tid = team_thread();
     const int lane = tid & 31, wid = tid / 32, g = lane >> 2, t = lane & 3;
@@ -324,25 +328,17 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
     const int64_t from = cut.start(part), until = cut.start(part + 1);
     int64_t at = from, base, b = run_of(a, starts, at, base);
     while (at < until) {
-        Seq s = seq_of<RB>(a, b);
-        for (int64_t w; at >= base + (w = static_cast<int64_t>(s.units) * s.blocks * a.kv_heads);) {
+        Seq s;
+        for (;; b++) {
+            s = seq_of<RB>(a, b);
+            const int64_t w = static_cast<int64_t>(s.units) * s.blocks * a.kv_heads;
+            if (at < base + w) break;
             base += w;
-            s = seq_of<RB>(a, ++b);
         }
         const int item = static_cast<int>(quotient(at - base, s.units));
         const int ua = static_cast<int>(at - base - static_cast<int64_t>(item) * s.units);
         const int ub = static_cast<int>(min(static_cast<int64_t>(s.units), ua + (until - at)));
         const int head = item / s.blocks, row0 = item % s.blocks * RB;
-        if (tid == 0) {
-            Note &note = notes[a.item_blocks ? b * a.item_blocks * a.kv_heads + item : part];
-            const int64_t start = at - ua, before = part > 0 ? cut.start(part - 1) : 0;
-            if (at == from && ua > 0 && before <= start) {
-                note = Note{static_cast<int>(cut.part_of(start + s.units - 1) - part) + 2, head, row0, s.count * a.share,
-                            s.first, 2 * (part - 1) + (before == start ? 0 : 1), part, 0};
-            } else if (a.item_blocks && ua == 0 && ub == s.units) {
-                note.pieces = 0;
-            }
-        }
 
         // This warp's units: ua + wid, ua + wid + WARPS, ...  Lanes 2j and
         // 2j + 1 find the two tiles of every 16th step from j on, so one pass
@@ -379,81 +375,101 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
             }
             issued++;
         };
-        while (issued < STAGES - 1 && issued < n_units) fetch(issued);
+        for (; issued < STAGES - 1 && issued < n_units;) fetch(issued);
+
 
         // Queries: column n of the block is row row0 + n of (query, shared
         // head).  Scaled by a power of two that takes the block's largest to
         // just under 2^15 and held as f16 (f32: two terms): exact for 16-bit
-        // types but for elements below 2^-29 of the largest.
-        uint32_t qf[QS][NT][D / 16][2];
-        float c2[NT][NG][2];
-        int all_lo = 0, all_hi = s.len;
-        float xq[NT][NG][W][8], top_q = 0.0f;
+        // types but for elements below 2^-29 of the largest.  The team's
+        // threads take eight channels each and leave them, in the order in
+        // which the products take them, in the stages that are filled last.
+        const auto q_at = [&](int row, int qs, int chunk) {
+            return reinterpret_cast<uint4 *>(smem + (row & 3) * S::RING + (STAGES - 1) * S::STAGE) +
+                   ((row >> 2) * QS + qs) * (D / 8) + chunk;
+        };
+        constexpr int EACH = (RB * D / 8 + 32 * WARPS - 1) / (32 * WARPS);
+        float xq[EACH][8];
+        uint32_t top_q = 0;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int r = row0 + 8 * nt + g;
-            const bool real = r < s.count * a.share;
-            const T *q = static_cast<const T *>(a.q);
-            if (real)
-                q += (s.first + r / a.share) * a.q_token + (static_cast<int64_t>(head) * a.share + r % a.share) * a.q_head;
-            float sum[NG];
+        for (int i = 0; i < EACH; i++) {
+            const int idx = tid + i * 32 * WARPS, row = idx / (D / 8), ch = idx % (D / 8) * 8, r = row0 + row;
+            if (idx >= RB * D / 8) break;  // whole warps
+            if (r < s.count * a.share) {
+                load8(static_cast<const T *>(a.q) + (s.first + r / a.share) * a.q_token +
+                          (static_cast<int64_t>(head) * a.share + r % a.share) * a.q_head + ch,
+                      a.vec, xq[i]);
+            } else {
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-                sum[gr] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    float(&x)[8] = xq[nt][gr][w];
-                    if (real) {
-                        load8(q + gr * G + (t * W + w) * 8, a.vec, x);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = 0.0f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        top_q = fmaxf(top_q, fabsf(x[e]));
-                        sum[gr] += x[e];
-                    }
-                }
-                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+                for (int e = 0; e < 8; e++) xq[i][e] = 0.0f;
             }
+            float sum = 0.0f, top = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-#pragma unroll
-                for (int gr = 0; gr < NG; gr++)
-                    c2[nt][gr][e] = __shfl_sync(0xffffffffu, sum[gr], (2 * t + e) * 4) * a.scale_log2;
-                const int2 sees = seen_by(a, s, row0 + 8 * nt + 2 * t + e);
-                all_lo = max(all_lo, sees.x);
-                all_hi = min(all_hi, sees.y);
+            for (int e = 0; e < 8; e++) {
+                sum += xq[i][e];
+                top = fmaxf(top, fabsf(xq[i][e]));
             }
+            top_q = max(top_q, __float_as_uint(top));
+#pragma unroll
+            for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (ch % G == 0) q_sums[team][row][ch / G] = sum;
         }
-        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
-        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-        const int top_exp = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top_q)) >> 23);
+        top_q = __reduce_max_sync(0xffffffffu, top_q);
+        if (lane == 0) q_tops[team][wid] = top_q;
+        team_sync();
+        const int top_exp = static_cast<int>(max(max(q_tops[team][0], q_tops[team][1]), max(q_tops[team][2], q_tops[team][3])) >> 23);
         const int up = top_exp > 0 ? max(-100, min(100, 14 + 127 - top_exp)) : 0;
-        const float up_mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
         // a code is c 2^-24 (c 2^-20 in the upper nibbles: those channels take q / 16)
         const float c1 = __uint_as_float(static_cast<uint32_t>(24 - up + 127) << 23) * a.scale_log2;
+        const float up_mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int idx = tid + i * 32 * WARPS, row = idx / (D / 8), chunk = idx % (D / 8);
+            if (idx >= RB * D / 8) break;
+            uint32_t high[4], low[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {  // channels k and k + 4
+                const float f = k & 1 ? up_mul * 0.0625f : up_mul;
+                const float u = xq[i][k] * f, v = xq[i][k + 4] * f;
+                high[k] = pack2(u, v);
+                const float2 r2 = unpack2(high[k]);
+                low[k] = pack2(u - r2.x, v - r2.y);
+            }
+            *q_at(row, 0, chunk) = make_uint4(high[0], high[1], high[2], high[3]);
+            if constexpr (S::F32) *q_at(row, 1, chunk) = make_uint4(low[0], low[1], low[2], low[3]);
+        }
+        fence_proxy_async_smem();
+        team_sync();
+        uint32_t qf[QS][NT][D / 16][2];
+        float c2[NT][NG][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++)
+            for (int gr = 0; gr < NG; gr++) {
 #pragma unroll
-                for (int w = 0; w < W; w++)
+                for (int qs = 0; qs < QS; qs++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
+                    for (int w = 0; w < W; w++) {
+                        const uint4 v = *q_at(8 * nt + g, qs, gr * (G / 8) + t * W + w);
+                        uint32_t(*f)[2] = &qf[qs][nt][gr * KS + 2 * w];
+                        f[0][0] = v.x, f[0][1] = v.y, f[1][0] = v.z, f[1][1] = v.w;
+                    }
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const float f = h ? up_mul * 0.0625f : up_mul;
-                            const float u = xq[nt][gr][w][2 * k + h] * f, v = xq[nt][gr][w][2 * k + h + 4] * f;
-                            const uint32_t p = pack2(u, v);
-                            qf[0][nt][gr * KS + 2 * w + k][h] = p;
-                            if constexpr (S::F32) {
-                                const float2 r2 = unpack2(p);
-                                qf[QS - 1][nt][gr * KS + 2 * w + k][h] = pack2(u - r2.x, v - r2.y);
-                            }
-                        }
+                for (int e = 0; e < 2; e++) c2[nt][gr][e] = q_sums[team][8 * nt + 2 * t + e][gr] * a.scale_log2;
+            }
+        team_sync();
+        // what every row of the block sees
+        const int all_lo = seen_by(a, s, row0 + RB - 1).x, all_hi = seen_by(a, s, row0).y;
+        if (tid == 0) {
+            Note &note = notes[a.item_blocks ? b * a.item_blocks * a.kv_heads + item : part];
+            const int64_t start = at - ua, before = part > 0 ? cut.start(part - 1) : 0;
+            if (at == from && ua > 0 && before <= start) {
+                note = Note{static_cast<int>(cut.part_of(start + s.units - 1) - part) + 2, head, row0, s.count * a.share,
+                            s.first, 2 * (part - 1) + (before == start ? 0 : 1), part, 0};
+            } else if (a.item_blocks && ua == 0 && ub == s.units) {
+                note.pieces = 0;
+            }
+        }
 
         // Weights are 2^(x - ref).  With vexp the exponent of the largest
         // value scale so far (below 2^(vexp - 14)), a weight times a scale
