@@ -51,7 +51,8 @@ struct AttnArgs {
 
 constexpr int UNIT = 32;     // keys of one step of a warp: two tiles
 constexpr int WARPS = 4;     // warps of a block; they take a piece's units in turn
-constexpr int MIN_UNITS = 4;  // units of a part at least (one for each warp)
+constexpr int PAD = 8;       // what starting a piece costs, in units of a team's work
+constexpr int MIN_PART = 4 + PAD;  // of a part at least: a unit for each warp
 
 struct Seq {
     int64_t first;         // its first row
@@ -98,7 +99,7 @@ __device__ __forceinline__ int2 seen_by(const AttnArgs &a, const Seq &s, int r) 
 template <int RB>
 __device__ __forceinline__ int64_t weight_of(const AttnArgs &a, int64_t b) {
     const Seq s = seq_of<RB>(a, b);
-    return static_cast<int64_t>(s.units) * s.blocks * a.kv_heads;
+    return static_cast<int64_t>(s.units + PAD) * s.blocks * a.kv_heads;
 }
 
 // a / b; 64-bit division, about 100 instructions, only where it is needed.  Not
@@ -108,8 +109,8 @@ __device__ __noinline__ int64_t quotient(int64_t a, int64_t b) {
     return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
 }
 
-// The units of all items (an item: a kv head's block of rows), one after the
-// other, are cut into n equal parts, one for each team of WARPS warps; part i
+// The units of all items (an item: a kv head's block of rows), each followed by
+// PAD that stand for its start, one after the other, are cut into n equal parts, one for each team of WARPS warps; part i
 // is that of team i / SMs of block i % SMs.  Teams of one block advance evenly.
 // Separate blocks on an SM do not (the SM issues for the oldest first): four
 // with equal parts ended after 162, 176, 196 and 217 us, the last ones alone.
@@ -118,7 +119,7 @@ struct Cut {
     int n, more;  // `each` units, the first `more` parts one more
     __device__ void divide(int64_t units, int parts) {
         total = units;
-        n = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(parts), total / MIN_UNITS)));
+        n = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(parts), total / MIN_PART)));
         each = quotient(total, n);
         more = static_cast<int>(total - each * n);
     }
@@ -331,12 +332,16 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
         Seq s;
         for (;; b++) {
             s = seq_of<RB>(a, b);
-            const int64_t w = static_cast<int64_t>(s.units) * s.blocks * a.kv_heads;
+            const int64_t w = static_cast<int64_t>(s.units + PAD) * s.blocks * a.kv_heads;
             if (at < base + w) break;
             base += w;
         }
-        const int item = static_cast<int>(quotient(at - base, s.units));
-        const int ua = static_cast<int>(at - base - static_cast<int64_t>(item) * s.units);
+        const int item = static_cast<int>(quotient(at - base, s.units + PAD));
+        const int ua = static_cast<int>(at - base - static_cast<int64_t>(item) * (s.units + PAD));
+        if (ua >= s.units) {
+            at += s.units + PAD - ua;
+            continue;
+        }
         const int ub = static_cast<int>(min(static_cast<int64_t>(s.units), ua + (until - at)));
         const int head = item / s.blocks, row0 = item % s.blocks * RB;
 
@@ -738,7 +743,7 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
         }
         fence_proxy_async_smem();  // the rings' next writers are bulk copies
         team_sync();
-        at += ub - ua;
+        at += ub < s.units ? ub - ua : s.units + PAD - ua;
     }
 }
 
@@ -828,7 +833,7 @@ struct Plan {
         const int64_t per_seq = (max_q * share + rb - 1) / rb;
         const int64_t blocks = std::min(per_seq * batch, (rows * share + rb - 1) / rb + batch);
         const double units = static_cast<double>(blocks) * kv_heads * static_cast<double>((max_keys + UNIT - 1) / UNIT + 1);
-        parts = static_cast<int64_t>(std::max(1.0, std::min(1.0 * at_once, units / MIN_UNITS + 1)));
+        parts = static_cast<int64_t>(std::max(1.0, std::min(1.0 * at_once, units / 4 + 1)));
         const bool by_item = per_seq * batch <= at_once / kv_heads;
         item_blocks = by_item ? static_cast<int>(per_seq) : 0;
         notes = by_item ? per_seq * batch * kv_heads : parts;
