@@ -425,18 +425,20 @@ ST_API st_status st_kv4_attn_workspace(st_handle *h, int64_t batch, int64_t rows
  * times - presence[r] for tokens in the history after its first prompt[r];
  * + the row's bias entries; -inf where the row's mask bit is 0.  The history is
  * tokens[starts[r] .. starts[r + 1]) (int32; others than 0 .. vocab - 1 are
- * skipped), the bias entries bias_starts[r] .. bias_starts[r + 1] of
+ * skipped; n_tokens in all), the bias entries bias_starts[r] .. bias_starts[r + 1] of
  * bias_tokens, bias_values (a token may occur twice: they are summed in order;
- * tokens outside the vocabulary are skipped).  mask int32 [masks, (vocab + 31)
+ * tokens outside the vocabulary are skipped; n_bias in all).  A row whose
+ * starts lead out of its list has none, and ST_INVALID_ARG at the next
+ * st_sync.  mask int32 [masks, (vocab + 31)
  * / 32], bit v % 32 of word v / 32; row r uses mask mask_rows[r] (negative:
  * none; at or past masks: none, and ST_INVALID_ARG at the next st_sync; NULL:
  * mask r).  Every array but logits and out may be NULL (prompt NULL: 0). */
 ST_API st_status st_logits_adjust(st_handle *h, const void *logits, int64_t ld, void *out, int64_t out_ld,
-                                  int64_t rows, int64_t vocab, const int32_t *tokens, const int32_t *starts,
-                                  const int32_t *prompt, const float *repetition, const float *presence,
-                                  const float *frequency, const int32_t *bias_tokens, const float *bias_values,
-                                  const int32_t *bias_starts, const int32_t *mask, int64_t masks,
-                                  const int32_t *mask_rows, int32_t dtype);
+                                  int64_t rows, int64_t vocab, const int32_t *tokens, int64_t n_tokens,
+                                  const int32_t *starts, const int32_t *prompt, const float *repetition,
+                                  const float *presence, const float *frequency, const int32_t *bias_tokens,
+                                  const float *bias_values, int64_t n_bias, const int32_t *bias_starts,
+                                  const int32_t *mask, int64_t masks, const int32_t *mask_rows, int32_t dtype);
 
 /* ---- kNN memory: 2-bit key scan fused with top-k ------------------------- */
 

@@ -198,9 +198,9 @@ extern "C" {
     pub fn st_kv4_attn_workspace(h: *mut st_handle, batch: i64, rows: i64, max_q: i64, max_keys: i64,
         heads: i32, kv_heads: i32, d: i32, bytes: *mut i64) -> st_status;
     pub fn st_logits_adjust(h: *mut st_handle, logits: *const c_void, ld: i64, out: *mut c_void, out_ld: i64,
-        rows: i64, vocab: i64, tokens: *const i32, starts: *const i32, prompt: *const i32,
+        rows: i64, vocab: i64, tokens: *const i32, n_tokens: i64, starts: *const i32, prompt: *const i32,
         repetition: *const f32, presence: *const f32, frequency: *const f32, bias_tokens: *const i32,
-        bias_values: *const f32, bias_starts: *const i32, mask: *const i32, masks: i64, mask_rows: *const i32,
+        bias_values: *const f32, n_bias: i64, bias_starts: *const i32, mask: *const i32, masks: i64, mask_rows: *const i32,
         dtype: i32) -> st_status;
 }
 

@@ -112,8 +112,8 @@ SIGNATURES = {
     "st_kv4_attn": (_st, [_h, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp,
                           _i64, _i64, _i64, _f32, _i32, _i32, _i32, _i32, _vp, _i64]),
     "st_kv4_attn_workspace": (_st, [_h, _i64, _i64, _i64, _i64, _i32, _i32, _i32, ctypes.POINTER(_i64)]),
-    "st_logits_adjust": (_st, [_h, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                               _i64, _vp, _i32]),
+    "st_logits_adjust": (_st, [_h, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                               _vp, _vp, _i64, _vp, _i32]),
     "st_avg_params": (_st, [_h, _vp, _i64, _vp]),
     "st_knn_search_sharded": (_st, [_h, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
 }

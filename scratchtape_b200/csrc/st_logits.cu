@@ -25,12 +25,13 @@ struct LogitsArgs {
     const int32_t *bias_tokens, *bias_starts;
     const float *bias_values;
     const int32_t *mask, *mask_rows;
-    int64_t masks;
-    int words, vec;
+    int64_t masks, n_tokens, n_bias;
+    int words, vec, copy;  // copy: out is not simply in
     int *status;
 };
 
-constexpr int CHUNK = 16384, THREADS = 512, HOLD = 8, LIST = 4096;
+constexpr int THREADS = 512, SLOTS = 8192, WINDOW = 2 * SLOTS, HASHED = SLOTS / 2, HOLD = HASHED / THREADS;
+constexpr int MASK_THREADS = 256, MASK_EACH = 4;
 
 // Four words of logits, -inf where their mask bits are 0.
 template <typename T>
@@ -47,157 +48,211 @@ __device__ __forceinline__ void mask_words(uint32_t (&w)[4], uint32_t bits) {
     }
 }
 
-// One block per (piece of a row, row).  A piece is CHUNK tokens from a 16-byte
-// boundary of the row's memory on; `shift` elements of the first one lie
-// before the row.  Few tokens of a piece occur in the history, so the block
-// looks through the history while the piece's logits are on their way to
-// registers: each token that occurs (or has a bias) is listed once and its
-// count cleared, then they are counted, and a thread for each listed token
-// computes its new logit.  The piece itself is only masked and stored; the
-// listed tokens' logits follow it.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) k_logits_adjust(const LogitsArgs a) {
-    constexpr int VEC = 16 / sizeof(T), EACH = CHUNK / VEC / THREADS;
-    extern __shared__ uint32_t cnt[];  // [CHUNK]: 2 n_said + (once in the prompt), in the end the new logit's bits
-    __shared__ uint32_t touched[CHUNK / 32], biased[CHUNK / 32];
-    __shared__ uint16_t list[LIST];
-    __shared__ int listed;
-    grid_dep_wait();
-    const int64_t r = blockIdx.y;
+__device__ __forceinline__ const uint32_t *mask_of(const LogitsArgs &a, int64_t r) {
+    if (!a.mask) return nullptr;
+    const int64_t m = a.mask_rows ? a.mask_rows[r] : r;
+    if (m >= a.masks) {
+        if (threadIdx.x == 0) set_status(a.status, DEV_BAD_ARG);
+        return nullptr;
+    }
+    return m >= 0 ? reinterpret_cast<const uint32_t *>(a.mask) + m * a.words : nullptr;
+}
+__device__ __forceinline__ bool allowed(const uint32_t *mask, int v) { return !mask || (mask[v / 32] >> (v % 32) & 1u); }
+
+// Row r's entries of `list`: from `at` on, n of them (none where starts leads out of it).
+__device__ __forceinline__ void run_of(const int32_t *list, const int32_t *starts, int64_t r, int64_t most, int *status,
+                                       int &at, int &n) {
+    at = n = 0;
+    if (!list) return;
+    const int from = starts[r], to = starts[r + 1];
+    if (from < 0 || to < from || to > most) {
+        if (threadIdx.x == 0) set_status(status, DEV_BAD_ARG);
+        return;
+    }
+    at = from;
+    n = to - from;
+}
+
+// Copies the vectors first, first + step, ... (EACH of them) of row r with the
+// mask applied.  Vector 0 starts at the last 16-byte boundary at or before the
+// row's memory.
+template <typename T, int EACH>
+__device__ __forceinline__ void mask_row(const LogitsArgs &a, int64_t r, const uint32_t *mask, int first, int step) {
+    constexpr int VEC = 16 / sizeof(T);
     const T *in = static_cast<const T *>(a.in) + r * a.ld;
     T *out = static_cast<T *>(a.out) + r * a.out_ld;
     const int shift = a.vec ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) % VEC) : 0;
-    const int v0 = static_cast<int>(blockIdx.x) * CHUNK - shift;  // the token of the piece's first element
-    if (v0 >= a.vocab) return;
-    const int s = a.tokens ? a.starts[r] : 0, e = a.tokens ? a.starts[r + 1] : 0;
-    const int bs = a.bias_tokens ? a.bias_starts[r] : 0, be = a.bias_tokens ? a.bias_starts[r + 1] : 0;
-    const int said = s + (a.prompt ? a.prompt[r] : 0);
-    int64_t mr = -1;
-    if (a.mask) {
-        mr = a.mask_rows ? a.mask_rows[r] : r;
-        if (mr >= a.masks) {
-            if (threadIdx.x == 0) set_status(a.status, DEV_BAD_ARG);
-            mr = -1;
-        }
-    }
-    const uint32_t *mask = mr >= 0 ? reinterpret_cast<const uint32_t *>(a.mask) + mr * a.words : nullptr;
-    uint32_t x[EACH][4];
+    uint4 x[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-        const int v = v0 + (i * THREADS + static_cast<int>(threadIdx.x)) * VEC;
-        if (a.vec && v >= 0 && v + VEC <= a.vocab) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(in + v);
-            x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
-        }
+        const int64_t v = static_cast<int64_t>(first + i * step) * VEC - shift;
+        if (a.vec && v >= 0 && v + VEC <= a.vocab) x[i] = *reinterpret_cast<const uint4 *>(in + v);
     }
-    const int low = max(v0, 0);
-    const uint32_t here = min(v0 + CHUNK, a.vocab) - low;
-    const auto place = [&](int token) {  // in the piece, or -1
-        return static_cast<uint32_t>(token - low) < here ? token - v0 : -1;
-    };
-    int held[HOLD];  // the history's first tokens, for both looks
-#pragma unroll
-    for (int k = 0; k < HOLD; k++) {
-        const int i = s + k * THREADS + static_cast<int>(threadIdx.x);
-        held[k] = i < e ? a.tokens[i] : -1;
-    }
-    if (threadIdx.x == 0) listed = 0;
-    for (int i = threadIdx.x; i < CHUNK / 32; i += THREADS) touched[i] = biased[i] = 0;
-    __syncthreads();
-    const auto touch = [&](int p) {
-        const uint32_t bit = 1u << (p & 31);
-        if (p >= 0 && !(atomicOr(&touched[p / 32], bit) & bit)) {
-            cnt[p] = 0;
-            const int at = atomicAdd(&listed, 1);
-            if (at < LIST) list[at] = static_cast<uint16_t>(p);
-        }
-    };
-#pragma unroll
-    for (int k = 0; k < HOLD; k++) touch(held[k] = place(held[k]));
-    for (int i = s + HOLD * THREADS + threadIdx.x; i < e; i += THREADS) touch(place(a.tokens[i]));
-    for (int i = bs + threadIdx.x; i < be; i += THREADS) {
-        const int p = place(a.bias_tokens[i]);
-        touch(p);
-        if (p >= 0) atomicOr(&biased[p / 32], 1u << (p % 32));
-    }
-    __syncthreads();
-    const auto count = [&](int p, int i) {
-        if (p >= 0) {
-            if (i >= said)
-                atomicAdd(&cnt[p], 2u);
-            else
-                atomicOr(&cnt[p], 1u);
-        }
-    };
-#pragma unroll
-    for (int k = 0; k < HOLD; k++) count(held[k], s + k * THREADS + static_cast<int>(threadIdx.x));
-    for (int i = s + HOLD * THREADS + threadIdx.x; i < e; i += THREADS) count(place(a.tokens[i]), i);
-    __syncthreads();
-    const float rep = a.repetition ? a.repetition[r] : 1.0f, pres = a.presence ? a.presence[r] : 0.0f,
-                freq = a.frequency ? a.frequency[r] : 0.0f;
-    // every listed token, or where they are more than the list holds, every bit
-    const bool whole = listed <= LIST;
-    const int many = whole ? listed : CHUNK;
-    const auto token_of = [&](int i) { return whole ? list[i] : touched[i / 32] >> (i % 32) & 1u ? i : -1; };
-    for (int i = threadIdx.x; i < many; i += THREADS) {
-        const int p = token_of(i);
-        if (p < 0) continue;
-        float y = to_f32(in[v0 + p]);
-        const uint32_t n = cnt[p];
-        if (n) y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-        if (n > 1) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n >> 1))), pres);
-        if (biased[p / 32] >> (p % 32) & 1u) {
-            float sum = 0.0f;
-            for (int j = bs; j < be; j++)
-                if (a.bias_tokens[j] == v0 + p) sum = __fadd_rn(sum, a.bias_values[j]);
-            y = __fadd_rn(y, sum);
-        }
-        if (mask && !(mask[(v0 + p) / 32] >> ((v0 + p) % 32) & 1u)) y = -INFINITY;
-        cnt[p] = __float_as_uint(y);
-    }
-    __syncthreads();  // all of the piece is read before any of it is written: out may be in
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-        const int v = v0 + (i * THREADS + static_cast<int>(threadIdx.x)) * VEC;
+        const int64_t v = static_cast<int64_t>(first + i * step) * VEC - shift;
         if (a.vec && v >= 0 && v + VEC <= a.vocab) {
-            if (mask) mask_words<T>(x[i], __funnelshift_r(mask[v / 32], mask[(v + VEC - 1) / 32], v % 32));
-            *reinterpret_cast<uint4 *>(out + v) = make_uint4(x[i][0], x[i][1], x[i][2], x[i][3]);
+            uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            if (mask) mask_words<T>(w, __funnelshift_r(mask[v / 32], mask[(v + VEC - 1) / 32], v % 32));
+            *reinterpret_cast<uint4 *>(out + v) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll 1
-            for (int k = max(0, -v); k < VEC && v + k < a.vocab; k++)
-                out[v + k] = mask && !(mask[(v + k) / 32] >> ((v + k) % 32) & 1u) ? from_f32<T>(-INFINITY) : in[v + k];
+            for (int64_t u = max(v, static_cast<int64_t>(0)); u < v + VEC && u < a.vocab; u++)
+                out[u] = allowed(mask, static_cast<int>(u)) ? in[u] : from_f32<T>(-INFINITY);
         }
     }
+}
+
+// All of the rows but for the tokens that k_logits_tokens adjusts afterwards:
+// a copy, -inf where the mask has a 0.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(MASK_THREADS) k_logits_mask(const LogitsArgs a) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t r = blockIdx.y;
+    mask_row<T, MASK_EACH>(a, r, mask_of(a, r), blockIdx.x * MASK_THREADS * MASK_EACH + threadIdx.x, MASK_THREADS);
+}
+
+// The tokens that occur in a row's history or have a bias: counted in shared
+// memory, then each logit (which the mask has left as it was) adjusted in
+// place.  Up to HASHED entries go through a hash table of SLOTS by one block;
+// longer histories are looked through by a block for each WINDOW of the
+// vocabulary, which counts it densely.  With one window the block has copied
+// its row itself.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) k_logits_tokens(const LogitsArgs a, int after_mask) {
+    constexpr int VEC = 16 / sizeof(T), BATCH = 8;
+    constexpr uint32_t BIASED = 1u << 31;
+    extern __shared__ uint32_t cnt[];  // 2 n_said + (once in the prompt) + BIASED; [SLOTS] and then keys, or [WINDOW]
+    int *key = reinterpret_cast<int *>(cnt + SLOTS);
+    // after the mask's launch, that one has waited for all before it
+    if (!after_mask) grid_dep_wait();
+    const int64_t r = blockIdx.x;
+    int s, n_hist, bs, n_bias;
+    run_of(a.tokens, a.starts, r, a.n_tokens, a.status, s, n_hist);
+    run_of(a.bias_tokens, a.bias_starts, r, a.n_bias, a.status, bs, n_bias);
+    const bool hashed = n_hist <= HASHED - n_bias;
+    const uint32_t *mask = mask_of(a, r);
+    if (!after_mask && a.copy)
+        for (int first = threadIdx.x; first * VEC < a.vocab + VEC; first += 2 * THREADS) mask_row<T, 2>(a, r, mask, first, THREADS);
+    if ((hashed && blockIdx.y > 0) || (n_hist <= 0 && n_bias <= 0)) return;
+    const int prompt = a.prompt ? a.prompt[r] : 0;
+    int held[HOLD];
+    if (hashed) {
+#pragma unroll
+        for (int k = 0; k < HOLD; k++) {
+            const int i = k * THREADS + static_cast<int>(threadIdx.x);
+            held[k] = i < n_hist ? a.tokens[s + i] : -1;
+        }
+    }
+    for (int i = threadIdx.x; i < WINDOW / 4; i += THREADS)
+        reinterpret_cast<uint4 *>(cnt)[i] = hashed && i >= SLOTS / 4 ? make_uint4(~0u, ~0u, ~0u, ~0u) : make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = threadIdx.x; i < many; i += THREADS)
-        if (const int p = token_of(i); p >= 0) out[v0 + p] = from_f32<T>(__uint_as_float(cnt[p]));
+    const int low = hashed ? 0 : blockIdx.y * WINDOW;
+    const uint32_t here = hashed ? a.vocab : min(WINDOW, a.vocab - low);
+    const auto place = [&](int token) {  // of its count; taken for it if it had none
+        if (!hashed) return static_cast<uint32_t>(token - low);
+        uint32_t p = static_cast<uint32_t>(token) * 2654435769u >> 19;
+        for (;; p = (p + 1) % SLOTS) {  // at most half full: ends
+            const int was = atomicCAS(&key[p], -1, token);
+            if (was == -1 || was == token) return p;
+        }
+    };
+    const auto add = [&](int token, uint32_t what) {  // 2: add; another bit: set
+        if (static_cast<uint32_t>(token - low) >= here) return;
+        const uint32_t p = place(token);
+        if (what == 2)
+            atomicAdd(&cnt[p], what);
+        else
+            atomicOr(&cnt[p], what);
+    };
+    if (hashed) {
+#pragma unroll
+        for (int k = 0; k < HOLD; k++)
+            add(held[k], k * THREADS + static_cast<int>(threadIdx.x) >= prompt ? 2u : 1u);
+    } else {
+        for (int i = threadIdx.x; i < n_hist; i += THREADS) add(a.tokens[s + i], i >= prompt ? 2u : 1u);
+    }
+    for (int i = threadIdx.x; i < n_bias; i += THREADS) add(a.bias_tokens[bs + i], BIASED);
+    const float rep = a.repetition ? a.repetition[r] : 1.0f, pres = a.presence ? a.presence[r] : 0.0f,
+                freq = a.frequency ? a.frequency[r] : 0.0f;
+    if (after_mask) grid_dep_wait();
+    __syncthreads();
+    T *out = static_cast<T *>(a.out) + r * a.out_ld;
+    const auto penalised = [&](float y, uint32_t n) {
+        if (n) y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+        if (n > 1) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, static_cast<float>(n >> 1))), pres);
+        return y;
+    };
+    // tokens with a bias, each by the thread of its first entry
+    for (int i = threadIdx.x; i < n_bias; i += THREADS) {
+        const int v = a.bias_tokens[bs + i];
+        if (static_cast<uint32_t>(v - low) >= here) continue;
+        float sum = 0.0f;
+        bool first = true;
+        for (int j = 0; j < n_bias; j++)
+            if (a.bias_tokens[bs + j] == v) {
+                first &= j >= i;
+                sum = __fadd_rn(sum, a.bias_values[bs + j]);
+            }
+        if (first && allowed(mask, v))
+            out[v] = from_f32<T>(__fadd_rn(penalised(to_f32(out[v]), cnt[place(v)] & ~BIASED), sum));
+    }
+    for (int i0 = threadIdx.x; i0 < (hashed ? SLOTS : WINDOW); i0 += BATCH * THREADS) {
+        int token[BATCH];
+        T before[BATCH];
+        uint32_t word[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {  // all loads on their way before any is used
+            const int i = i0 + k * THREADS;
+            token[k] = hashed ? key[i] : cnt[i] ? low + i : -1;
+            const int at = max(token[k], 0);
+            before[k] = out[at];
+            word[k] = mask ? mask[at / 32] : ~0u;
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+            if (token[k] < 0 || !(word[k] >> (token[k] % 32) & 1u)) continue;  // none, or -inf already
+            const uint32_t n = cnt[i0 + k * THREADS];
+            if (!(n & BIASED)) out[token[k]] = from_f32<T>(penalised(to_f32(before[k]), n));
+        }
+    }
 }
 
 template <typename T>
-st_status launch(st_handle *h, const LogitsArgs &a) {
-    constexpr int VEC = 16 / sizeof(T);
-    const dim3 grid(static_cast<unsigned>((a.vocab + (a.vec ? VEC - 1 : 0) + CHUNK - 1) / CHUNK),
-                    static_cast<unsigned>(a.rows));
-    const size_t smem = sizeof(uint32_t) * CHUNK;
-    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_logits_adjust<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+st_status launch(st_handle *h, LogitsArgs a) {
+    constexpr int VEC = 16 / sizeof(T), PIECE = MASK_THREADS * MASK_EACH * VEC;
+    const int windows = (a.vocab + WINDOW - 1) / WINDOW;
+    a.copy = a.mask || a.in != a.out || a.ld != a.out_ld;
+    const int apart = windows > 1 && a.copy;
+    const bool all_hashed = a.n_tokens + a.n_bias <= HASHED;
+    if (apart) {
+        const dim3 grid(static_cast<unsigned>((a.vocab + VEC - 1 + PIECE - 1) / PIECE), static_cast<unsigned>(a.rows));
+        ST_CHECK_CUDA(h, st_launch_dependent(h, k_logits_mask<T>, grid, dim3(MASK_THREADS), 0, a));
+        if (st_status s = st_after_launch(h, "k_logits_mask"); s != ST_OK) return s;
+    }
+    if ((windows > 1 || !a.copy) && !a.tokens && !a.bias_tokens) return ST_OK;
+    const size_t smem = sizeof(uint32_t) * WINDOW;
+    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_logits_tokens<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           static_cast<int>(smem)));
-    ST_CHECK_CUDA(h, st_launch_dependent(h, k_logits_adjust<T>, grid, dim3(THREADS), smem, a));
-    return st_after_launch(h, "k_logits_adjust");
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_logits_tokens<T>, dim3(static_cast<unsigned>(a.rows), all_hashed ? 1 : windows),
+                                         dim3(THREADS), smem, a, apart));
+    return st_after_launch(h, "k_logits_tokens");
 }
 
 }  // namespace
 
 extern "C" st_status st_logits_adjust(st_handle *h, const void *logits, int64_t ld, void *out, int64_t out_ld,
-                                      int64_t rows, int64_t vocab, const int32_t *tokens, const int32_t *starts,
-                                      const int32_t *prompt, const float *repetition, const float *presence,
-                                      const float *frequency, const int32_t *bias_tokens, const float *bias_values,
-                                      const int32_t *bias_starts, const int32_t *mask, int64_t masks,
-                                      const int32_t *mask_rows, int32_t dtype) {
+                                      int64_t rows, int64_t vocab, const int32_t *tokens, int64_t n_tokens,
+                                      const int32_t *starts, const int32_t *prompt, const float *repetition,
+                                      const float *presence, const float *frequency, const int32_t *bias_tokens,
+                                      const float *bias_values, int64_t n_bias, const int32_t *bias_starts,
+                                      const int32_t *mask, int64_t masks, const int32_t *mask_rows, int32_t dtype) {
     if (!h) return ST_INVALID_ARG;
-    if (rows < 0 || vocab < 1 || ld < vocab || out_ld < vocab || dtype < ST_F32 || dtype > ST_BF16)
+    if (rows < 0 || vocab < 1 || ld < vocab || out_ld < vocab || n_tokens < 0 || n_bias < 0 || dtype < ST_F32 || dtype > ST_BF16)
         return h->fail(ST_INVALID_ARG, "st_logits_adjust: bad arguments");
-    if (rows > 65535 || vocab > (1 << 30))
-        return h->fail(ST_UNSUPPORTED_SHAPE, "st_logits_adjust: at most 65535 rows and 2^30 tokens");
+    if (rows > 65535 || vocab > (1 << 28))
+        return h->fail(ST_UNSUPPORTED_SHAPE, "st_logits_adjust: at most 65535 rows and 2^28 tokens");
     if (rows == 0) return ST_OK;
     if (!logits || !out) return h->fail(ST_INVALID_ARG, "st_logits_adjust: null logits or out");
     if (tokens && !starts) return h->fail(ST_INVALID_ARG, "st_logits_adjust: a history needs its starts");
@@ -212,7 +267,7 @@ extern "C" st_status st_logits_adjust(st_handle *h, const void *logits, int64_t 
     const uintptr_t in0 = reinterpret_cast<uintptr_t>(logits), out0 = reinterpret_cast<uintptr_t>(out);
     const int vec = (in0 - out0) % 16 == 0 && (rows == 1 || (ld - out_ld) * size % 16 == 0) && in0 % size == 0;
     const LogitsArgs a = {logits, out, ld, out_ld, rows, static_cast<int>(vocab), tokens, starts, prompt, repetition,
-                          presence, frequency, bias_tokens, bias_starts, bias_values, mask, mask_rows, masks,
-                          static_cast<int>((vocab + 31) / 32), vec, h->d_status};
+                          presence, frequency, bias_tokens, bias_starts, bias_values, mask, mask_rows, masks, n_tokens, n_bias,
+                          static_cast<int>((vocab + 31) / 32), vec, 1, h->d_status};
     return dtype == ST_F32 ? launch<float>(h, a) : dtype == ST_F16 ? launch<__half>(h, a) : launch<__nv_bfloat16>(h, a);
 }

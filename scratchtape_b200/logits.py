@@ -55,7 +55,9 @@ def adjust(logits: torch.Tensor, tokens=None, starts=None, prompt=None, repetiti
         _of(words, torch.int32, logits, "mask", (words.shape[0], (vocab + 31) // 32))
         _of(which, torch.int32, logits, "mask rows", (rows,))
     handle(logits.device).call("st_logits_adjust", ptr(logits), max(vocab, logits.stride(0)), ptr(out),
-                               max(vocab, out.stride(0)), rows, vocab, ptr(tokens), ptr(starts), ptr(prompt),
-                               ptr(repetition), ptr(presence), ptr(frequency), ptr(ids), ptr(values), ptr(at),
+                               max(vocab, out.stride(0)), rows, vocab, ptr(tokens),
+                               0 if tokens is None else tokens.numel(), ptr(starts), ptr(prompt), ptr(repetition),
+                               ptr(presence), ptr(frequency), ptr(ids), ptr(values),
+                               0 if ids is None else ids.numel(), ptr(at),
                                ptr(words), 0 if words is None else words.shape[0], ptr(which), _DTYPES[logits.dtype])
     return out
