@@ -18,6 +18,8 @@ struct AppendArgs {
     uint8_t *data;
     int64_t n_pages, n;
     int page, kv_heads, heads, rotary, interleaved;
+    int vec;     // rows start on a boundary of a lane's channels
+    int tiles;   // values go by tiles of tokens, in warps of their own
     const void *k, *v, *q;
     void *q_out;
     int64_t k_token, k_head, v_token, v_head, q_token, q_head;
@@ -28,151 +30,394 @@ struct AppendArgs {
     int *status;
 };
 
-// Channels c .. c + E of x, rotated by the position whose cos / sin rows are
-// given (rows of rotary / 2).
-template <typename T, int E>
-__device__ __forceinline__ void load_rotated(const T *x, int c, const float *cs, const float *sn, int rotary,
-                                             int interleaved, float (&out)[E]) {
+// How a head's d = 32 E channels lie in a warp.  Plain: lane l has channels
+// E l ..., Split: it has (E / 2) l ... of the lower half and the same of the upper
+// one, so that both channels of a pair (i, i + d / 2) are in one lane.
+template <int D, bool SPLIT>
+__device__ __forceinline__ int channel(int lane, int e) {
+    constexpr int E = D / 32;
+    return !SPLIT ? lane * E + e : e < E / 2 ? lane * (E / 2) + e : D / 2 + lane * (E / 2) + e - E / 2;
+}
+
+template <typename T, int D, bool SPLIT>
+__device__ __forceinline__ void load_head(const T *x, int lane, int vec, float (&out)[D / 32]) {
+    constexpr int E = D / 32, RUN = SPLIT ? E / 2 : E;  // consecutive channels
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int ch = c + e;
-        const float own = to_f32(x[ch]);
-        out[e] = own;
-        if (ch < rotary) {
-            const int half = rotary / 2;
-            const bool first = interleaved ? (ch & 1) == 0 : ch < half;
-            const int i = interleaved ? ch >> 1 : (first ? ch : ch - half);
-            const float other = to_f32(x[interleaved ? ch ^ 1 : (first ? ch + half : ch - half)]);
-            const float p = __fmul_rn(own, cs[i]), r = __fmul_rn(other, sn[i]);
-            out[e] = first ? __fsub_rn(p, r) : __fadd_rn(p, r);
+    for (int e0 = 0; e0 < E; e0 += RUN) {
+        const T *p = x + channel<D, SPLIT>(lane, e0);
+        alignas(16) T v[RUN];
+        if (vec) {
+            if constexpr (RUN * sizeof(T) == 16) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+            if constexpr (RUN * sizeof(T) == 8) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+            if constexpr (RUN * sizeof(T) == 4) *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(p);
+            if constexpr (RUN * sizeof(T) == 2) v[0] = p[0];
+        } else {
+#pragma unroll
+            for (int e = 0; e < RUN; e++) v[e] = p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < RUN; e++) out[e0 + e] = to_f32(v[e]);
+    }
+}
+
+// Writes a lane's channels; out is packed, so its rows are aligned.
+template <typename T, int D, bool SPLIT>
+__device__ __forceinline__ void store_head(T *out, int lane, const float (&x)[D / 32]) {
+    constexpr int E = D / 32, RUN = SPLIT ? E / 2 : E;
+#pragma unroll
+    for (int e0 = 0; e0 < E; e0 += RUN) {
+        T *p = out + channel<D, SPLIT>(lane, e0);
+        alignas(16) T v[RUN];
+#pragma unroll
+        for (int e = 0; e < RUN; e++) v[e] = from_f32<T>(x[e0 + e]);
+        if constexpr (RUN * sizeof(T) == 16) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v);
+        if constexpr (RUN * sizeof(T) == 8) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(v);
+        if constexpr (RUN * sizeof(T) == 4) *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(v);
+        if constexpr (RUN * sizeof(T) == 2) p[0] = v[0];
+    }
+}
+
+// Quantises a head by groups of G: the lane's codes, and for each of its
+// channels its group's {scale, zero}.
+template <int D, int G, bool SPLIT>
+__device__ __forceinline__ void quantise(float (&x)[D / 32], uint32_t (&code)[D / 32], __half2 (&meta)[2]) {
+    constexpr int E = D / 32;
+    constexpr int SETS = SPLIT && G < D ? 2 : 1, PER = E / SETS;  // a lane's channels are of SETS groups
+    constexpr int LANES = G / PER < 32 ? G / PER : 32;             // lanes of a group
+#pragma unroll
+    for (int set = 0; set < SETS; set++) {
+        float lo = 65504.0f, hi = -65504.0f;
+#pragma unroll
+        for (int e = set * PER; e < (set + 1) * PER; e++) {
+            x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const __half zero = __float2half_rn(lo);
+        const float z = __half2float(zero);
+        const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f));
+        const float s = __half2float(scale);
+        const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+#pragma unroll
+        for (int e = set * PER; e < (set + 1) * PER; e++)
+            code[e] = static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], z), inv)), 0.0f), 15.0f));
+        meta[set] = __halves2half2(scale, zero);
+    }
+    if (SETS == 1) meta[1] = meta[0];
+}
+
+// Writes a head's codes and groups' {scale, zero} as token r of tile t.
+template <int D, int G, bool SPLIT>
+__device__ __forceinline__ void write_codes(uint8_t *t, int r, int lane, bool value, const uint32_t (&code)[D / 32],
+                                            const __half2 (&meta)[2]) {
+    constexpr int E = D / 32, RUN = SPLIT ? E / 2 : E;
+#pragma unroll
+    for (int e0 = 0; e0 < E; e0 += RUN) {
+        const int c = channel<D, SPLIT>(lane, e0);
+        uint8_t *row = value ? t + kv4_val(D) + c / 2 * 16 + kv4_col(r)
+                             : t + (c / G) * 8 * G + r * (G / 2) + (c % G) / 2;
+        if constexpr (RUN == 1) {  // a byte is two lanes' channels
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, code[e0], 1);
+            if (lane % 2 == 0) *row = static_cast<uint8_t>(code[e0] | other << 4);
+        } else {
+#pragma unroll
+            for (int e = 0; e < RUN; e += 2)
+                row[value ? e / 2 * 16 : e / 2] = static_cast<uint8_t>(code[e0 + e] | code[e0 + e + 1] << 4);
+        }
+        if (c % G == 0)
+            *reinterpret_cast<__half2 *>(t + (value ? kv4_vmeta(D, G) : kv4_kmeta(D)) + ((c / G) * 16 + r) * 4) =
+                meta[e0 ? 1 : 0];
+    }
+}
+
+// A slot's page and its place there; 32-bit division wherever it will do.
+struct Place {
+    int64_t page;
+    int off;
+    __device__ Place(int64_t slot, int size) {
+        if (slot >> 32 == 0) {
+            page = static_cast<uint32_t>(slot) / static_cast<uint32_t>(size);
+            off = static_cast<int>(static_cast<uint32_t>(slot) - static_cast<uint32_t>(page) * size);
+        } else {
+            page = slot / size;
+            off = static_cast<int>(slot - page * size);
         }
     }
-}
+};
 
-// Quantises a warp's d = 32 E channels (lane's E consecutive ones in x) by
-// groups of G; the lane's codes go to code[], its group's pair to meta.
-template <int E, int G>
-__device__ __forceinline__ void quantise(float (&x)[E], uint32_t (&code)[E], __half2 &meta) {
-    float lo = 65504.0f, hi = -65504.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-    }
-#pragma unroll
-    for (int o = G / E / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const __half zero = __float2half_rn(lo);
-    const float z = __half2float(zero);
-    const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f));
-    const float s = __half2float(scale);
-    const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        code[e] = static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], z), inv)), 0.0f), 15.0f));
-    meta = __halves2half2(scale, zero);
-}
+constexpr int HEADS = 4;  // heads of a token whose loads a warp has under way together
 
-// One warp per (token, head) of the keys, the values and (when rotated) the
-// queries.
-template <typename T, int D, int G>
-__global__ void k_kv4_append(const AppendArgs a) {
+// One warp per (token, HEADS heads of its keys, queries and -- unless they go
+// by tiles -- values); the token's row of cos and sin is read once for them.
+// SPLIT: the rotation is of pairs (i, i + d / 2); else any.
+template <typename T, int D, int G, bool SPLIT>
+__device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, int lane) {
     constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t w = blockIdx.x * static_cast<int64_t>(blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t per = 2 * a.kv_heads + (a.q ? a.heads : 0);
-    if (w >= a.n * per) return;
-    const int64_t i = w / per;
-    const int j = static_cast<int>(w % per);
-    const int c = lane * E;
+    const int n_q = a.q ? a.heads : 0, n_v = a.tiles ? 0 : a.kv_heads, all = a.kv_heads + n_q + n_v;
+    const uint32_t per = (all + HEADS - 1) / HEADS, token = w / per;
+    const int64_t i = token;
+    const int h0 = static_cast<int>(w - token * per) * HEADS;
     int64_t pos = 0;
+    const int64_t slot = a.slots[i];
+    bool keep = slot >= 0, bad = slot >= a.n_pages * a.page, turn = a.rotary > 0;
     if (a.rotary) {
         pos = a.positions[i];
         if (pos < 0 || pos >= a.n_positions) {
-            if (lane == 0) set_status(a.status, DEV_BAD_ARG);
-            return;
+            bad = true;
+            turn = false;
         }
     }
+    if (bad && lane == 0) set_status(a.status, DEV_BAD_ARG);
+    keep &= !bad;
     const float *cs = a.cos + pos * (a.rotary / 2), *sn = a.sin + pos * (a.rotary / 2);
-    float x[E];
-    if (j >= 2 * a.kv_heads) {
-        const int64_t head = j - 2 * a.kv_heads;
-        load_rotated<T, E>(static_cast<const T *>(a.q) + i * a.q_token + head * a.q_head, c, cs, sn, a.rotary,
-                           a.interleaved, x);
-        T *out = static_cast<T *>(a.q_out) + (i * a.heads + head) * D + c;
+    float x[HEADS][E], c[E], s[E];
+    const T *src[HEADS];
 #pragma unroll
-        for (int e = 0; e < E; e++) out[e] = from_f32<T>(x[e]);
-        return;
+    for (int j = 0; j < HEADS; j++) {
+        const int64_t h = h0 + j;
+        src[j] = h < a.kv_heads         ? static_cast<const T *>(a.k) + i * a.k_token + h * a.k_head
+                 : h < a.kv_heads + n_q ? static_cast<const T *>(a.q) + i * a.q_token + (h - a.kv_heads) * a.q_head
+                                        : static_cast<const T *>(a.v) + i * a.v_token + (h - a.kv_heads - n_q) * a.v_head;
+        if (h < all) load_head<T, D, SPLIT>(src[j], lane, a.vec, x[j]);
     }
-    const int64_t slot = a.slots[i];
-    if (slot < 0) return;
-    if (slot >= a.n_pages * a.page) {
-        if (lane == 0) set_status(a.status, DEV_BAD_ARG);
-        return;
-    }
-    const bool value = j >= a.kv_heads;
-    const int head = value ? j - a.kv_heads : j;
-    if (value)
-        load_rotated<T, E>(static_cast<const T *>(a.v) + i * a.v_token + head * a.v_head, c, cs, sn, 0, 0, x);
-    else
-        load_rotated<T, E>(static_cast<const T *>(a.k) + i * a.k_token + head * a.k_head, c, cs, sn, a.rotary,
-                           a.interleaved, x);
-    uint32_t code[E];
-    __half2 meta;
-    quantise<E, G>(x, code, meta);
-    const int off = static_cast<int>(slot % a.page), r = off & 15;
-    const int64_t tile = ((slot / a.page) * a.kv_heads + head) * (a.page / 16) + off / 16;
-    uint8_t *t = a.data + tile * kv4_tile_bytes(D, G);
-    if (value) {
+    if (turn) {
 #pragma unroll
-        for (int e = 0; e < E; e += 2)
-            t[kv4_val(D) + (c + e) / 2 * 16 + kv4_col(r)] = static_cast<uint8_t>(code[e] | code[e + 1] << 4);
-    } else {
-        uint8_t *row = t + (c / G) * 8 * G + r * (G / 2) + (c % G) / 2;
-#pragma unroll
-        for (int e = 0; e < E; e += 2) row[e / 2] = static_cast<uint8_t>(code[e] | code[e + 1] << 4);
+        for (int e = 0; e < E; e++) {
+            const int ch = channel<D, SPLIT>(lane, e), half = a.rotary / 2;
+            if (SPLIT) {
+                if (e < E / 2) c[e] = cs[ch], s[e] = sn[ch];
+            } else if (ch < a.rotary) {
+                const int at = a.interleaved ? ch >> 1 : ch < half ? ch : ch - half;
+                c[e] = cs[at], s[e] = sn[at];
+            }
+        }
     }
-    if (c % G == 0)
-        *reinterpret_cast<__half2 *>(t + (value ? kv4_vmeta(D, G) : kv4_kmeta(D)) + ((c / G) * 16 + r) * 4) = meta;
+    const Place at(keep ? slot : 0, a.page);
+    const int r = at.off & 15;
+    const int64_t tile0 = at.page * a.kv_heads * (a.page / 16) + at.off / 16;
+#pragma unroll
+    for (int j = 0; j < HEADS; j++) {
+        const int h = h0 + j;
+        if (h >= all) break;
+        const bool value = h >= a.kv_heads + n_q;
+        if (turn && !value) {
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int e = 0; e < E / 2; e++) {
+                    const float u = x[j][e], v = x[j][e + E / 2];
+                    x[j][e] = __fsub_rn(__fmul_rn(u, c[e]), __fmul_rn(v, s[e]));
+                    x[j][e + E / 2] = __fadd_rn(__fmul_rn(v, c[e]), __fmul_rn(u, s[e]));
+                }
+            } else {
+                float y[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const int ch = lane * E + e, half = a.rotary / 2;
+                    y[e] = x[j][e];
+                    if (ch < a.rotary) {
+                        const bool first = a.interleaved ? (ch & 1) == 0 : ch < half;
+                        const float other = a.interleaved ? x[j][e ^ 1] : to_f32(src[j][first ? ch + half : ch - half]);
+                        const float p = __fmul_rn(x[j][e], c[e]), q = __fmul_rn(other, s[e]);
+                        y[e] = first ? __fsub_rn(p, q) : __fadd_rn(p, q);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < E; e++) x[j][e] = y[e];
+            }
+        }
+        if (h >= a.kv_heads && !value) {
+            if (turn) store_head<T, D, SPLIT>(static_cast<T *>(a.q_out) + (i * a.heads + h - a.kv_heads) * D, lane, x[j]);
+        } else if (keep) {
+            uint32_t code[E];
+            __half2 meta[2];
+            quantise<D, G, SPLIT>(x[j], code, meta);
+            const int head = value ? h - a.kv_heads - n_q : h;
+            write_codes<D, G, SPLIT>(a.data + (tile0 + head * static_cast<int64_t>(a.page / 16)) * kv4_tile_bytes(D, G), r,
+                                     lane, value, code, meta);
+        }
+    }
 }
 
-// One warp per (slot, head): the lane's E channels of the key and the value.
+// One warp per (16 tokens of the list, head): their values.  Where tokens
+// fill a tile in order, the warp in whose 16 it begins holds the codes of all
+// its 16 until it can write whole rows of the tile; other tokens' codes are
+// written byte by byte.
 template <typename T, int D, int G>
-__global__ void k_kv4_read(const uint8_t *data, int64_t n_pages, int page, int kv_heads, const int64_t *slots,
-                           int64_t n, T *k, T *v, int *status) {
+__device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, int lane) {
     constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t w = blockIdx.x * static_cast<int64_t>(blockDim.x / 32) + threadIdx.x / 32;
-    if (w >= n * kv_heads) return;
-    const int64_t i = w / kv_heads;
-    const int head = static_cast<int>(w % kv_heads), c = lane * E;
-    int64_t slot = slots[i];
-    if (slot >= n_pages * page) {
-        if (lane == 0) set_status(status, DEV_BAD_ARG);
-        slot = -1;
-    }
-    T *ko = k + w * D + c, *vo = v + w * D + c;
-    if (slot < 0) {
+    const uint32_t sixteen = w / a.kv_heads;
+    const int64_t i0 = sixteen * 16ll;
+    const int head = static_cast<int>(w - sixteen * a.kv_heads);
+    const int64_t most = a.n_pages * a.page;
+    const auto slot_of = [&](int64_t i) -> int64_t {
+        if (i < 0 || i >= a.n) return -1;
+        const int64_t pos = a.rotary ? a.positions[i] : 0;  // a token without a position is left out whole
+        return pos < 0 || (a.rotary && pos >= a.n_positions) ? -1 : a.slots[i];
+    };
+    // bits: token i0 - 15 + x of the list starts a tile; its follower's slot is the next one
+    const int64_t s0 = slot_of(i0 - 15 + lane), s1 = slot_of(i0 + 17 + lane);
+    int64_t n0 = __shfl_down_sync(0xffffffffu, s0, 1), n1 = __shfl_down_sync(0xffffffffu, s1, 1);
+    const int64_t s1_first = __shfl_sync(0xffffffffu, s1, 0);
+    if (lane == 31) n0 = s1_first, n1 = -1;
+    const auto bits = [&](bool low, bool high) {
+        return static_cast<uint64_t>(__ballot_sync(0xffffffffu, low)) |
+               static_cast<uint64_t>(__ballot_sync(0xffffffffu, high)) << 32;
+    };
+    uint64_t run = bits(s0 >= 0 && n0 == s0 + 1, s1 >= 0 && n1 == s1 + 1);
+    run &= run >> 1, run &= run >> 2, run &= run >> 4, run &= run >> 7;  // 15 followers in order
+    const uint64_t starts = run & bits(s0 >= 0 && s0 % 16 == 0 && s0 + 15 < most, s1 >= 0 && s1 % 16 == 0 && s1 + 15 < most);
+    uint64_t inside = starts;
+    inside |= inside << 1, inside |= inside << 2, inside |= inside << 4, inside |= inside << 8;
+    const uint32_t begins = static_cast<uint32_t>(starts >> 15) & 0xffffu, alone = ~static_cast<uint32_t>(inside >> 15) & 0xffffu;
+    const T *v = static_cast<const T *>(a.v) + head * a.v_head;
+    const auto tile_of = [&](int64_t slot) {
+        const Place at(slot, a.page);
+        return a.data + ((at.page * a.kv_heads + head) * (a.page / 16) + at.off / 16) * kv4_tile_bytes(D, G);
+    };
+    if (begins) {
+        const int64_t i = i0 + __ffs(begins) - 1;
+        uint8_t *t = tile_of(a.slots[i]);
+        uint32_t row[E / 2][4];
 #pragma unroll
-        for (int e = 0; e < E; e++) ko[e] = vo[e] = from_f32<T>(0.0f);
+        for (int b = 0; b < 4; b++) {  // tokens 2b, 2b + 8, 2b + 1, 2b + 9 make word b of a row
+            float x[4][E];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                load_head<T, D, false>(v + (i + 2 * b + (k & 1) * 8 + (k >> 1)) * a.v_token, lane, a.vec, x[k]);
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) row[e][b] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t code[E];
+                __half2 meta[2];
+                quantise<D, G, false>(x[k], code, meta);
+#pragma unroll
+                for (int e = 0; e < E / 2; e++) row[e][b] |= (code[2 * e] | code[2 * e + 1] << 4) << (8 * k);
+                if (lane * E % G == 0)
+                    *reinterpret_cast<__half2 *>(t + kv4_vmeta(D, G) +
+                                                 ((lane * E / G) * 16 + 2 * b + (k & 1) * 8 + (k >> 1)) * 4) = meta[0];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E / 2; e++)
+            *reinterpret_cast<uint4 *>(t + kv4_val(D) + (lane * (E / 2) + e) * 16) =
+                make_uint4(row[e][0], row[e][1], row[e][2], row[e][3]);
+    }
+    for (uint32_t left = alone; left; left &= left - 1) {
+        const int64_t i = i0 + __ffs(left) - 1, slot = slot_of(i);
+        if (slot < 0) continue;
+        if (slot >= most) {
+            if (lane == 0) set_status(a.status, DEV_BAD_ARG);
+            continue;
+        }
+        float x[E];
+        uint32_t code[E];
+        __half2 meta[2];
+        load_head<T, D, false>(v + i * a.v_token, lane, a.vec, x);
+        quantise<D, G, false>(x, code, meta);
+        write_codes<D, G, false>(tile_of(slot), static_cast<int>(slot % 16), lane, true, code, meta);
+    }
+}
+
+template <typename T, int D, int G, bool SPLIT>
+__global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a, uint32_t token_warps) {
+    const uint32_t w = blockIdx.x * 4u + threadIdx.x / 32;
+    const int lane = threadIdx.x & 31;
+    grid_dep_wait();
+    if (w < token_warps)
+        append_token<T, D, G, SPLIT>(a, w, lane);
+    else if (a.tiles && w - token_warps < (a.n + 15) / 16 * a.kv_heads)
+        append_values<T, D, G>(a, w - token_warps, lane);
+}
+
+// One warp per (16 slots of the list, head).  A lane takes E consecutive
+// channels; where the 16 slots are a tile's in order, it reads its rows of value
+// codes whole (16 bytes each) for all of them, else byte by byte.
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(128) k_kv4_read(const uint8_t *data, int64_t n_pages, int page, int kv_heads,
+                                                  const int64_t *slots, int64_t n, T *k, T *v, int *status) {
+    constexpr int E = D / 32, TILE = kv4_tile_bytes(D, G);
+    const int lane = threadIdx.x & 31;
+    const uint32_t w = blockIdx.x * 4u + threadIdx.x / 32, sixteen = w / kv_heads;
+    const int64_t i0 = sixteen * 16ll;
+    grid_dep_wait();
+    if (i0 >= n) return;
+    const int head = static_cast<int>(w - sixteen * kv_heads), c = lane * E, count = static_cast<int>(min(n - i0, static_cast<int64_t>(16)));
+    int64_t mine = lane < count ? slots[i0 + lane] : -1;
+    if (mine >= n_pages * page) {
+        set_status(status, DEV_BAD_ARG);
+        mine = -1;
+    }
+    const int64_t first = __shfl_sync(0xffffffffu, mine, 0);
+    const bool whole = __all_sync(0xffffffffu, lane >= 16 || (first >= 0 && first % 16 == 0 && mine == first + lane));
+    const auto tile_of = [&](int64_t slot) {
+        const Place at(slot, page);
+        return data + ((at.page * kv_heads + head) * (page / 16) + at.off / 16) * TILE;
+    };
+    T *ko = k + (i0 * kv_heads + head) * D, *vo = v + (i0 * kv_heads + head) * D;
+    const int64_t step = static_cast<int64_t>(kv_heads) * D;
+    // codes of E channels in the low bits of `key`; of the values, byte `col` of the rows
+    const auto emit = [&](int j, uint32_t key, const uint32_t (&val)[E / 2], __half2 km, __half2 vm) {
+        const float2 a = __half22float2(km), b = __half22float2(vm);
+        float x[E], y[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            x[e] = fmaf(static_cast<float>(key >> (4 * e) & 15u), a.x, a.y);
+            y[e] = fmaf(static_cast<float>(val[e / 2] >> (4 * (e % 2)) & 15u), b.x, b.y);
+        }
+        store_head<T, D, false>(ko + j * step, lane, x);
+        store_head<T, D, false>(vo + j * step, lane, y);
+    };
+    if (whole) {
+        const uint8_t *t = tile_of(first);
+        uint4 rows[E / 2];
+#pragma unroll
+        for (int e = 0; e < E / 2; e++) rows[e] = reinterpret_cast<const uint4 *>(t + kv4_val(D))[lane * (E / 2) + e];
+        const uint8_t *kc = t + (c / G) * 8 * G + (c % G) / 2;
+        const __half2 *km = reinterpret_cast<const __half2 *>(t + kv4_kmeta(D)) + (c / G) * 16;
+        const __half2 *vm = reinterpret_cast<const __half2 *>(t + kv4_vmeta(D, G)) + (c / G) * 16;
+        uint32_t key[16];
+        __half2 ka[16], va[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            key[j] = E == 4 ? *reinterpret_cast<const uint16_t *>(kc + j * (G / 2)) : kc[j * (G / 2)];
+            ka[j] = km[j];
+            va[j] = vm[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            uint32_t val[E / 2];
+            const int col = kv4_col(j);
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) {
+                const uint32_t word[4] = {rows[e].x, rows[e].y, rows[e].z, rows[e].w};
+                val[e] = word[col / 4] >> (8 * (col % 4));
+            }
+            emit(j, key[j], val, ka[j], va[j]);
+        }
         return;
     }
-    const int off = static_cast<int>(slot % page), r = off & 15;
-    const int64_t tile = ((slot / page) * kv_heads + head) * (page / 16) + off / 16;
-    const uint8_t *t = data + tile * kv4_tile_bytes(D, G);
-    const float2 km = __half22float2(*reinterpret_cast<const __half2 *>(t + kv4_kmeta(D) + ((c / G) * 16 + r) * 4));
-    const float2 vm = __half22float2(*reinterpret_cast<const __half2 *>(t + kv4_vmeta(D, G) + ((c / G) * 16 + r) * 4));
-    const uint8_t *kr = t + (c / G) * 8 * G + r * (G / 2) + (c % G) / 2;
+    for (int j = 0; j < count; j++) {
+        const int64_t slot = __shfl_sync(0xffffffffu, mine, j);
+        uint32_t key = 0, val[E / 2] = {};
+        __half2 km = __floats2half2_rn(0.0f, 0.0f), vm = km;
+        if (slot >= 0) {
+            const uint8_t *t = tile_of(slot);
+            const int r = static_cast<int>(slot % 16);
+            km = *reinterpret_cast<const __half2 *>(t + kv4_kmeta(D) + ((c / G) * 16 + r) * 4);
+            vm = *reinterpret_cast<const __half2 *>(t + kv4_vmeta(D, G) + ((c / G) * 16 + r) * 4);
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-        const uint32_t kb = kr[e / 2], vb = t[kv4_val(D) + (c + e) / 2 * 16 + kv4_col(r)];
-        ko[e] = from_f32<T>(fmaf(static_cast<float>(kb & 15), km.x, km.y));
-        ko[e + 1] = from_f32<T>(fmaf(static_cast<float>(kb >> 4), km.x, km.y));
-        vo[e] = from_f32<T>(fmaf(static_cast<float>(vb & 15), vm.x, vm.y));
-        vo[e + 1] = from_f32<T>(fmaf(static_cast<float>(vb >> 4), vm.x, vm.y));
+            for (int e = 0; e < E / 2; e++) {
+                key |= static_cast<uint32_t>(t[(c / G) * 8 * G + r * (G / 2) + (c % G) / 2 + e]) << (8 * e);
+                val[e] = t[kv4_val(D) + (c / 2 + e) * 16 + kv4_col(r)];
+            }
+        }
+        emit(j, key, val, km, vm);
     }
 }
 
@@ -196,11 +441,28 @@ st_status by_shape(int dtype, int d, int group, Args &&...args) {
 
 template <typename T, int D, int G>
 struct AppendLaunch {
-    static st_status run(st_handle *h, const AppendArgs &a) {
-        const int64_t warps = a.n * (2 * a.kv_heads + (a.q ? a.heads : 0));
-        const int64_t blocks = (warps + 3) / 4;
-        if (blocks > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_append: too many tokens");
-        k_kv4_append<T, D, G><<<static_cast<unsigned>(blocks), 128, 0, h->stream>>>(a);
+    static st_status run(st_handle *h, AppendArgs a) {
+        constexpr int E = D / 32;
+        const bool split = a.rotary == D && !a.interleaved;
+        // accesses of a lane's channels at once where every row starts on their boundary
+        const auto fits = [&](const void *p, int64_t token, int64_t head) {
+            return reinterpret_cast<uintptr_t>(p) % (E * sizeof(T)) == 0 && token % E == 0 && head % E == 0;
+        };
+        a.vec = fits(a.k, a.k_token, a.k_head) && fits(a.v, a.v_token, a.v_head) &&
+                (!a.q || fits(a.q, a.q_token, a.q_head));
+        // Single tokens of many sequences have no tiles to fill; from some hundreds
+        // of tokens on there are enough warps when 16 tokens share one.
+        a.tiles = a.n >= 512;
+        const int64_t all = a.kv_heads + (a.q ? a.heads : 0) + (a.tiles ? 0 : a.kv_heads);
+        const int64_t token_warps = a.n * ((all + HEADS - 1) / HEADS);
+        const int64_t warps = token_warps + (a.tiles ? (a.n + 15) / 16 * a.kv_heads : 0), blocks = (warps + 3) / 4;
+        if (warps > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_append: too many tokens");
+        if (split)
+            ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_append<T, D, G, true>, dim3(static_cast<unsigned>(blocks)),
+                                                 dim3(128), 0, a, static_cast<uint32_t>(token_warps)));
+        else
+            ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_append<T, D, G, false>, dim3(static_cast<unsigned>(blocks)),
+                                                 dim3(128), 0, a, static_cast<uint32_t>(token_warps)));
         return st_after_launch(h, "k_kv4_append");
     }
 };
@@ -209,10 +471,11 @@ template <typename T, int D, int G>
 struct ReadLaunch {
     static st_status run(st_handle *h, const uint8_t *data, int64_t n_pages, int page, int kv_heads,
                          const int64_t *slots, int64_t n, void *k, void *v) {
-        const int64_t blocks = (n * kv_heads + 3) / 4;
-        if (blocks > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_read: too many tokens");
-        k_kv4_read<T, D, G><<<static_cast<unsigned>(blocks), 128, 0, h->stream>>>(
-            data, n_pages, page, kv_heads, slots, n, static_cast<T *>(k), static_cast<T *>(v), h->d_status);
+        const int64_t warps = (n + 15) / 16 * kv_heads;
+        if (warps > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_read: too many tokens");
+        ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_read<T, D, G>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128),
+                                             0, data, n_pages, page, kv_heads, slots, n, static_cast<T *>(k),
+                                             static_cast<T *>(v), h->d_status));
         return st_after_launch(h, "k_kv4_read");
     }
 };
@@ -238,7 +501,7 @@ extern "C" st_status st_kv4_append(st_handle *h, void *data, int64_t n_pages, in
     if (q && (!q_out || heads < 1 || rotary == 0))
         return h->fail(ST_INVALID_ARG, "st_kv4_append: queries are only rotated: they need q_out and a rotation");
     cudaSetDevice(h->device);
-    const AppendArgs a = {static_cast<uint8_t *>(data), n_pages, n, page, kv_heads, heads, rotary, interleaved, k, v,
+    const AppendArgs a = {static_cast<uint8_t *>(data), n_pages, n, page, kv_heads, heads, rotary, interleaved, 0, 0, k, v,
                           q, q_out, k_token, k_head, v_token, v_head, q_token, q_head, cos, sin, positions,
                           n_positions, slots, h->d_status};
     return by_shape<AppendLaunch>(dtype, d, group, h, a);
