@@ -39,14 +39,14 @@ __device__ __forceinline__ int channel(int lane, int e) {
     return !SPLIT ? lane * E + e : e < E / 2 ? lane * (E / 2) + e : D / 2 + lane * (E / 2) + e - E / 2;
 }
 
-template <typename T, int D, bool SPLIT>
-__device__ __forceinline__ void load_head(const T *x, int lane, int vec, float (&out)[D / 32]) {
+template <typename T, int D, bool SPLIT, bool VEC>
+__device__ __forceinline__ void load_head(const T *x, int lane, float (&out)[D / 32]) {
     constexpr int E = D / 32, RUN = SPLIT ? E / 2 : E;  // consecutive channels
 #pragma unroll
     for (int e0 = 0; e0 < E; e0 += RUN) {
         const T *p = x + channel<D, SPLIT>(lane, e0);
         alignas(16) T v[RUN];
-        if (vec) {
+        if constexpr (VEC) {
             if constexpr (RUN * sizeof(T) == 16) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
             if constexpr (RUN * sizeof(T) == 8) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
             if constexpr (RUN * sizeof(T) == 4) *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(p);
@@ -150,42 +150,24 @@ struct Place {
     }
 };
 
-constexpr int HEADS = 4;  // heads of a token whose loads a warp has under way together
+enum Role { KEYS, QUERIES, VALUES };
 
-// One warp per (token, HEADS heads of its keys, queries and -- unless they go
-// by tiles -- values); the token's row of cos and sin is read once for them.
-// SPLIT: the rotation is of pairs (i, i + d / 2); else any.
-template <typename T, int D, int G, bool SPLIT>
-__device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, int lane) {
+// HEADS heads of one token from h0 on (of `all`): rotated by its row of cos and
+// sin, which is read once for them, and stored (queries) or quantised into
+// the token's tile.  SPLIT: the rotation is of pairs (i, i + d / 2); else any.
+// tile: the token's in the first head; null: not kept.
+template <typename T, int D, int G, bool SPLIT, bool VEC, int HEADS, Role ROLE>
+__device__ __forceinline__ void append_heads(const AppendArgs &a, const T *src, int64_t head_step, int h0, int all,
+                                             T *q_out, uint8_t *tile, int r, bool turn, const float *cs,
+                                             const float *sn, int lane) {
     constexpr int E = D / 32;
-    const int n_q = a.q ? a.heads : 0, n_v = a.tiles ? 0 : a.kv_heads, all = a.kv_heads + n_q + n_v;
-    const uint32_t per = (all + HEADS - 1) / HEADS, token = w / per;
-    const int64_t i = token;
-    const int h0 = static_cast<int>(w - token * per) * HEADS;
-    int64_t pos = 0;
-    const int64_t slot = a.slots[i];
-    bool keep = slot >= 0, bad = slot >= a.n_pages * a.page, turn = a.rotary > 0;
-    if (a.rotary) {
-        pos = a.positions[i];
-        if (pos < 0 || pos >= a.n_positions) {
-            bad = true;
-            turn = false;
-        }
-    }
-    if (bad && lane == 0) set_status(a.status, DEV_BAD_ARG);
-    keep &= !bad;
-    const float *cs = a.cos + pos * (a.rotary / 2), *sn = a.sin + pos * (a.rotary / 2);
+    const int64_t tile_step = a.page / 16 * kv4_tile_bytes(D, G);
     float x[HEADS][E], c[E], s[E];
-    const T *src[HEADS];
+    src += h0 * head_step;
 #pragma unroll
-    for (int j = 0; j < HEADS; j++) {
-        const int64_t h = h0 + j;
-        src[j] = h < a.kv_heads         ? static_cast<const T *>(a.k) + i * a.k_token + h * a.k_head
-                 : h < a.kv_heads + n_q ? static_cast<const T *>(a.q) + i * a.q_token + (h - a.kv_heads) * a.q_head
-                                        : static_cast<const T *>(a.v) + i * a.v_token + (h - a.kv_heads - n_q) * a.v_head;
-        if (h < all) load_head<T, D, SPLIT>(src[j], lane, a.vec, x[j]);
-    }
-    if (turn) {
+    for (int j = 0; j < HEADS; j++)
+        if (h0 + j < all) load_head<T, D, SPLIT, VEC>(src + j * head_step, lane, x[j]);
+    if (ROLE != VALUES && turn) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const int ch = channel<D, SPLIT>(lane, e), half = a.rotary / 2;
@@ -197,15 +179,12 @@ __device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, in
             }
         }
     }
-    const Place at(keep ? slot : 0, a.page);
-    const int r = at.off & 15;
-    const int64_t tile0 = at.page * a.kv_heads * (a.page / 16) + at.off / 16;
+    if (ROLE != QUERIES) tile += h0 * tile_step;
+    if (ROLE == QUERIES) q_out += h0 * D;
 #pragma unroll
     for (int j = 0; j < HEADS; j++) {
-        const int h = h0 + j;
-        if (h >= all) break;
-        const bool value = h >= a.kv_heads + n_q;
-        if (turn && !value) {
+        if (h0 + j >= all) break;
+        if (ROLE != VALUES && turn) {
             if constexpr (SPLIT) {
 #pragma unroll
                 for (int e = 0; e < E / 2; e++) {
@@ -221,7 +200,8 @@ __device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, in
                     y[e] = x[j][e];
                     if (ch < a.rotary) {
                         const bool first = a.interleaved ? (ch & 1) == 0 : ch < half;
-                        const float other = a.interleaved ? x[j][e ^ 1] : to_f32(src[j][first ? ch + half : ch - half]);
+                        const float other =
+                            a.interleaved ? x[j][e ^ 1] : to_f32(src[j * head_step + (first ? ch + half : ch - half)]);
                         const float p = __fmul_rn(x[j][e], c[e]), q = __fmul_rn(other, s[e]);
                         y[e] = first ? __fsub_rn(p, q) : __fadd_rn(p, q);
                     }
@@ -230,24 +210,56 @@ __device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, in
                 for (int e = 0; e < E; e++) x[j][e] = y[e];
             }
         }
-        if (h >= a.kv_heads && !value) {
-            if (turn) store_head<T, D, SPLIT>(static_cast<T *>(a.q_out) + (i * a.heads + h - a.kv_heads) * D, lane, x[j]);
-        } else if (keep) {
+        if constexpr (ROLE == QUERIES) {
+            store_head<T, D, SPLIT>(q_out + j * D, lane, x[j]);
+        } else {
             uint32_t code[E];
             __half2 meta[2];
             quantise<D, G, SPLIT>(x[j], code, meta);
-            const int head = value ? h - a.kv_heads - n_q : h;
-            write_codes<D, G, SPLIT>(a.data + (tile0 + head * static_cast<int64_t>(a.page / 16)) * kv4_tile_bytes(D, G), r,
-                                     lane, value, code, meta);
+            write_codes<D, G, SPLIT>(tile + j * tile_step, r, lane, ROLE == VALUES, code, meta);
         }
     }
+}
+
+// One warp per (token, HEADS heads of its queries, its keys or -- unless they go
+// by tiles -- its values).
+template <typename T, int D, int G, bool SPLIT, bool VEC, int HEADS>
+__device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, int lane) {
+    const uint32_t nq = a.q ? (a.heads + HEADS - 1) / HEADS : 0, nk = (a.kv_heads + HEADS - 1) / HEADS;
+    const uint32_t per = nq + nk + (a.tiles ? 0 : nk), token = w / per;
+    const int64_t i = token;
+    int job = static_cast<int>(w - token * per);
+    const int64_t slot = a.slots[i], pos = a.rotary ? a.positions[i] : 0;
+    const bool placed = !a.rotary || (pos >= 0 && pos < a.n_positions), keep = placed && slot >= 0 && slot < a.n_pages * a.page;
+    if ((!placed || slot >= a.n_pages * a.page) && lane == 0) set_status(a.status, DEV_BAD_ARG);
+    const bool turn = a.rotary > 0 && placed;
+    const float *cs = a.cos + pos * (a.rotary / 2), *sn = a.sin + pos * (a.rotary / 2);
+    if (job < static_cast<int>(nq)) {
+        if (turn)
+            append_heads<T, D, G, SPLIT, VEC, HEADS, QUERIES>(a, static_cast<const T *>(a.q) + i * a.q_token, a.q_head,
+                                                              job * HEADS, a.heads,
+                                                              static_cast<T *>(a.q_out) + i * a.heads * D, nullptr, 0, true,
+                                                              cs, sn, lane);
+        return;
+    }
+    if (!keep) return;
+    job -= nq;
+    const Place at(slot, a.page);
+    uint8_t *tile = a.data + (at.page * a.kv_heads * (a.page / 16) + at.off / 16) * kv4_tile_bytes(D, G);
+    if (job < static_cast<int>(nk))
+        append_heads<T, D, G, SPLIT, VEC, HEADS, KEYS>(a, static_cast<const T *>(a.k) + i * a.k_token, a.k_head, job * HEADS,
+                                                       a.kv_heads, nullptr, tile, at.off & 15, turn, cs, sn, lane);
+    else
+        append_heads<T, D, G, SPLIT, VEC, HEADS, VALUES>(a, static_cast<const T *>(a.v) + i * a.v_token, a.v_head,
+                                                         (job - static_cast<int>(nk)) * HEADS, a.kv_heads, nullptr, tile,
+                                                         at.off & 15, false, cs, sn, lane);
 }
 
 // One warp per (16 tokens of the list, head): their values.  Where tokens
 // fill a tile in order, the warp in whose 16 it begins holds the codes of all
 // its 16 until it can write whole rows of the tile; other tokens' codes are
 // written byte by byte.
-template <typename T, int D, int G>
+template <typename T, int D, int G, bool VEC>
 __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, int lane) {
     constexpr int E = D / 32;
     const uint32_t sixteen = w / a.kv_heads;
@@ -288,7 +300,7 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, i
             float x[4][E];
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                load_head<T, D, false>(v + (i + 2 * b + (k & 1) * 8 + (k >> 1)) * a.v_token, lane, a.vec, x[k]);
+                load_head<T, D, false, VEC>(v + (i + 2 * b + (k & 1) * 8 + (k >> 1)) * a.v_token, lane, x[k]);
 #pragma unroll
             for (int e = 0; e < E / 2; e++) row[e][b] = 0;
 #pragma unroll
@@ -318,21 +330,28 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, i
         float x[E];
         uint32_t code[E];
         __half2 meta[2];
-        load_head<T, D, false>(v + i * a.v_token, lane, a.vec, x);
+        load_head<T, D, false, VEC>(v + i * a.v_token, lane, x);
         quantise<D, G, false>(x, code, meta);
         write_codes<D, G, false>(tile_of(slot), static_cast<int>(slot % 16), lane, true, code, meta);
     }
 }
 
-template <typename T, int D, int G, bool SPLIT>
+template <typename T, int D, int G, bool SPLIT, int HEADS>
 __global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a, uint32_t token_warps) {
     const uint32_t w = blockIdx.x * 4u + threadIdx.x / 32;
     const int lane = threadIdx.x & 31;
     grid_dep_wait();
-    if (w < token_warps)
-        append_token<T, D, G, SPLIT>(a, w, lane);
-    else if (a.tiles && w - token_warps < (a.n + 15) / 16 * a.kv_heads)
-        append_values<T, D, G>(a, w - token_warps, lane);
+    if (w < token_warps) {
+        if (a.vec)
+            append_token<T, D, G, SPLIT, true, HEADS>(a, w, lane);
+        else
+            append_token<T, D, G, SPLIT, false, HEADS>(a, w, lane);
+    } else if (a.tiles && w - token_warps < (a.n + 15) / 16 * a.kv_heads) {
+        if (a.vec)
+            append_values<T, D, G, true>(a, w - token_warps, lane);
+        else
+            append_values<T, D, G, false>(a, w - token_warps, lane);
+    }
 }
 
 // One warp per (16 slots of the list, head).  A lane takes E consecutive
@@ -450,19 +469,20 @@ struct AppendLaunch {
         };
         a.vec = fits(a.k, a.k_token, a.k_head) && fits(a.v, a.v_token, a.v_head) &&
                 (!a.q || fits(a.q, a.q_token, a.q_head));
-        // Single tokens of many sequences have no tiles to fill; from some hundreds
-        // of tokens on there are enough warps when 16 tokens share one.
+        // Single tokens of many sequences have no tiles to fill, and few tokens want
+        // many warps; from some hundreds of tokens on a warp does more.
         a.tiles = a.n >= 512;
-        const int64_t all = a.kv_heads + (a.q ? a.heads : 0) + (a.tiles ? 0 : a.kv_heads);
-        const int64_t token_warps = a.n * ((all + HEADS - 1) / HEADS);
+        if (split) return a.tiles ? launch<true, 8>(h, a) : launch<true, 4>(h, a);
+        return a.tiles ? launch<false, 8>(h, a) : launch<false, 4>(h, a);
+    }
+    template <bool SPLIT, int HEADS>
+    static st_status launch(st_handle *h, const AppendArgs &a) {
+        const int64_t nk = (a.kv_heads + HEADS - 1) / HEADS, nq = a.q ? (a.heads + HEADS - 1) / HEADS : 0;
+        const int64_t token_warps = a.n * (nq + nk + (a.tiles ? 0 : nk));
         const int64_t warps = token_warps + (a.tiles ? (a.n + 15) / 16 * a.kv_heads : 0), blocks = (warps + 3) / 4;
         if (warps > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_append: too many tokens");
-        if (split)
-            ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_append<T, D, G, true>, dim3(static_cast<unsigned>(blocks)),
-                                                 dim3(128), 0, a, static_cast<uint32_t>(token_warps)));
-        else
-            ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_append<T, D, G, false>, dim3(static_cast<unsigned>(blocks)),
-                                                 dim3(128), 0, a, static_cast<uint32_t>(token_warps)));
+        ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_append<T, D, G, SPLIT, HEADS>, dim3(static_cast<unsigned>(blocks)),
+                                             dim3(128), 0, a, static_cast<uint32_t>(token_warps)));
         return st_after_launch(h, "k_kv4_append");
     }
 };

@@ -131,8 +131,10 @@ struct Cut {
 };
 
 __device__ __forceinline__ int team_thread() { return threadIdx.x % (32 * WARPS); }
-// A barrier for the team's warps.
+// A barrier for the team's warps (each whole: it counts a warp for every time
+// that some of its lanes arrive).
 __device__ __forceinline__ void team_sync() {
+    __syncwarp();
     asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.x / (32 * WARPS) + 1), "n"(32 * WARPS) : "memory");
 }
 
