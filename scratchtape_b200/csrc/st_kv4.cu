@@ -39,13 +39,18 @@ __device__ __forceinline__ int channel(int lane, int e) {
     return !SPLIT ? lane * E + e : e < E / 2 ? lane * (E / 2) + e : D / 2 + lane * (E / 2) + e - E / 2;
 }
 
+template <typename T, int D>
+struct alignas(16) Raw {
+    T v[D / 32];
+};
+
 template <typename T, int D, bool SPLIT, bool VEC>
-__device__ __forceinline__ void load_head(const T *x, int lane, float (&out)[D / 32]) {
+__device__ __forceinline__ void load_raw(const T *x, int lane, Raw<T, D> &raw) {
     constexpr int E = D / 32, RUN = SPLIT ? E / 2 : E;  // consecutive channels
 #pragma unroll
     for (int e0 = 0; e0 < E; e0 += RUN) {
         const T *p = x + channel<D, SPLIT>(lane, e0);
-        alignas(16) T v[RUN];
+        T *v = raw.v + e0;
         if constexpr (VEC) {
             if constexpr (RUN * sizeof(T) == 16) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
             if constexpr (RUN * sizeof(T) == 8) *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
@@ -55,9 +60,12 @@ __device__ __forceinline__ void load_head(const T *x, int lane, float (&out)[D /
 #pragma unroll
             for (int e = 0; e < RUN; e++) v[e] = p[e];
         }
-#pragma unroll
-        for (int e = 0; e < RUN; e++) out[e0 + e] = to_f32(v[e]);
     }
+}
+template <typename T, int D>
+__device__ __forceinline__ void from_raw(const Raw<T, D> &raw, float (&out)[D / 32]) {
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) out[e] = to_f32(raw.v[e]);
 }
 
 // Writes a lane's channels; out is packed, so its rows are aligned.
@@ -162,11 +170,12 @@ __device__ __forceinline__ void append_heads(const AppendArgs &a, const T *src, 
                                              const float *sn, int lane) {
     constexpr int E = D / 32;
     const int64_t tile_step = a.page / 16 * kv4_tile_bytes(D, G);
-    float x[HEADS][E], c[E], s[E];
+    Raw<T, D> raw[HEADS];
+    float c[E], s[E];
     src += h0 * head_step;
 #pragma unroll
     for (int j = 0; j < HEADS; j++)
-        if (h0 + j < all) load_head<T, D, SPLIT, VEC>(src + j * head_step, lane, x[j]);
+        if (h0 + j < all) load_raw<T, D, SPLIT, VEC>(src + j * head_step, lane, raw[j]);
     if (ROLE != VALUES && turn) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
@@ -184,38 +193,40 @@ __device__ __forceinline__ void append_heads(const AppendArgs &a, const T *src, 
 #pragma unroll
     for (int j = 0; j < HEADS; j++) {
         if (h0 + j >= all) break;
+        float x[E];
+        from_raw(raw[j], x);
         if (ROLE != VALUES && turn) {
             if constexpr (SPLIT) {
 #pragma unroll
                 for (int e = 0; e < E / 2; e++) {
-                    const float u = x[j][e], v = x[j][e + E / 2];
-                    x[j][e] = __fsub_rn(__fmul_rn(u, c[e]), __fmul_rn(v, s[e]));
-                    x[j][e + E / 2] = __fadd_rn(__fmul_rn(v, c[e]), __fmul_rn(u, s[e]));
+                    const float u = x[e], v = x[e + E / 2];
+                    x[e] = __fsub_rn(__fmul_rn(u, c[e]), __fmul_rn(v, s[e]));
+                    x[e + E / 2] = __fadd_rn(__fmul_rn(v, c[e]), __fmul_rn(u, s[e]));
                 }
             } else {
                 float y[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     const int ch = lane * E + e, half = a.rotary / 2;
-                    y[e] = x[j][e];
+                    y[e] = x[e];
                     if (ch < a.rotary) {
                         const bool first = a.interleaved ? (ch & 1) == 0 : ch < half;
                         const float other =
-                            a.interleaved ? x[j][e ^ 1] : to_f32(src[j * head_step + (first ? ch + half : ch - half)]);
-                        const float p = __fmul_rn(x[j][e], c[e]), q = __fmul_rn(other, s[e]);
+                            a.interleaved ? x[e ^ 1] : to_f32(src[j * head_step + (first ? ch + half : ch - half)]);
+                        const float p = __fmul_rn(x[e], c[e]), q = __fmul_rn(other, s[e]);
                         y[e] = first ? __fsub_rn(p, q) : __fadd_rn(p, q);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < E; e++) x[j][e] = y[e];
+                for (int e = 0; e < E; e++) x[e] = y[e];
             }
         }
         if constexpr (ROLE == QUERIES) {
-            store_head<T, D, SPLIT>(q_out + j * D, lane, x[j]);
+            store_head<T, D, SPLIT>(q_out + j * D, lane, x);
         } else {
             uint32_t code[E];
             __half2 meta[2];
-            quantise<D, G, SPLIT>(x[j], code, meta);
+            quantise<D, G, SPLIT>(x, code, meta);
             write_codes<D, G, SPLIT>(tile + j * tile_step, r, lane, ROLE == VALUES, code, meta);
         }
     }
@@ -255,102 +266,101 @@ __device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, in
                                                          at.off & 15, false, cs, sn, lane);
 }
 
-// One warp per (16 tokens of the list, head): their values.  Where tokens
-// fill a tile in order, the warp in whose 16 it begins holds the codes of all
-// its 16 until it can write whole rows of the tile; other tokens' codes are
-// written byte by byte.
+// One warp per (16 places of the list, head): the values of the tiles that
+// begin there.  Token i of slot s belongs to the tile that begins at place i -
+// s % 16, on the understanding that its neighbours in the list are its
+// neighbours there; so the 31 tokens from the first place on hold all of the
+// 16 places' tiles, whole ones and those that the list cuts or leaves gaps in.
+// A tile's codes are gathered in registers: a whole row is one 16-byte store,
+// four tokens of a word one of 4 bytes, and others go byte by byte.
 template <typename T, int D, int G, bool VEC>
 __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, int lane) {
     constexpr int E = D / 32;
     const uint32_t sixteen = w / a.kv_heads;
-    const int64_t i0 = sixteen * 16ll;
+    const int64_t i0 = sixteen * 16ll - 16, i = i0 + lane, most = a.n_pages * a.page;
     const int head = static_cast<int>(w - sixteen * a.kv_heads);
-    const int64_t most = a.n_pages * a.page;
-    const auto slot_of = [&](int64_t i) -> int64_t {
-        if (i < 0 || i >= a.n) return -1;
+    int64_t slot = -1;
+    if (i >= 0 && i < a.n) {
         const int64_t pos = a.rotary ? a.positions[i] : 0;  // a token without a position is left out whole
-        return pos < 0 || (a.rotary && pos >= a.n_positions) ? -1 : a.slots[i];
-    };
-    // bits: token i0 - 15 + x of the list starts a tile; its follower's slot is the next one
-    const int64_t s0 = slot_of(i0 - 15 + lane), s1 = slot_of(i0 + 17 + lane);
-    int64_t n0 = __shfl_down_sync(0xffffffffu, s0, 1), n1 = __shfl_down_sync(0xffffffffu, s1, 1);
-    const int64_t s1_first = __shfl_sync(0xffffffffu, s1, 0);
-    if (lane == 31) n0 = s1_first, n1 = -1;
-    const auto bits = [&](bool low, bool high) {
-        return static_cast<uint64_t>(__ballot_sync(0xffffffffu, low)) |
-               static_cast<uint64_t>(__ballot_sync(0xffffffffu, high)) << 32;
-    };
-    uint64_t run = bits(s0 >= 0 && n0 == s0 + 1, s1 >= 0 && n1 == s1 + 1);
-    run &= run >> 1, run &= run >> 2, run &= run >> 4, run &= run >> 7;  // 15 followers in order
-    const uint64_t starts = run & bits(s0 >= 0 && s0 % 16 == 0 && s0 + 15 < most, s1 >= 0 && s1 % 16 == 0 && s1 + 15 < most);
-    uint64_t inside = starts;
-    inside |= inside << 1, inside |= inside << 2, inside |= inside << 4, inside |= inside << 8;
-    const uint32_t begins = static_cast<uint32_t>(starts >> 15) & 0xffffu, alone = ~static_cast<uint32_t>(inside >> 15) & 0xffffu;
+        if (pos >= 0 && (!a.rotary || pos < a.n_positions)) slot = a.slots[i];
+        if (slot >= most) slot = -1;  // reported by the keys' warp
+    }
+    const int begin = lane - static_cast<int>(slot & 15);  // its tile's place from i0 on
+    const int64_t tile = slot >> 4;
+    uint32_t left = __ballot_sync(0xffffffffu, slot >= 0 && begin >= 0 && begin < 16);
     const T *v = static_cast<const T *>(a.v) + head * a.v_head;
-    const auto tile_of = [&](int64_t slot) {
-        const Place at(slot, a.page);
-        return a.data + ((at.page * a.kv_heads + head) * (a.page / 16) + at.off / 16) * kv4_tile_bytes(D, G);
-    };
-    if (begins) {
-        const int64_t i = i0 + __ffs(begins) - 1;
-        uint8_t *t = tile_of(a.slots[i]);
+    while (left) {
+        const int one = __ffs(left) - 1, at = __shfl_sync(0xffffffffu, begin, one);
+        const int64_t its = __shfl_sync(0xffffffffu, tile, one);
+        const uint32_t members = __ballot_sync(0xffffffffu, slot >= 0 && begin == at && tile == its);
+        left &= ~members;
+        const uint32_t have = members >> at & 0xffffu;  // bit r: its token r is here, at place i0 + at + r
+        const T *src = v + (i0 + at) * a.v_token;
+        const Place place(its * 16, a.page);
+        uint8_t *t = a.data + ((place.page * a.kv_heads + head) * (a.page / 16) + place.off / 16) * kv4_tile_bytes(D, G);
+        uint8_t *codes = t + kv4_val(D) + lane * (E / 2) * 16;
         uint32_t row[E / 2][4];
+        Raw<T, D> raw[8];
 #pragma unroll
         for (int b = 0; b < 4; b++) {  // tokens 2b, 2b + 8, 2b + 1, 2b + 9 make word b of a row
-            float x[4][E];
+            if (b % 2 == 0) {  // eight tokens' loads under way together
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                load_head<T, D, false, VEC>(v + (i + 2 * b + (k & 1) * 8 + (k >> 1)) * a.v_token, lane, x[k]);
+                for (int k = 0; k < 8; k++)
+                    if (have >> (2 * b + k % 4 + k / 4 * 8) & 1u)
+                        load_raw<T, D, false, VEC>(src + (2 * b + k % 4 + k / 4 * 8) * a.v_token, lane, raw[k]);
+            }
 #pragma unroll
             for (int e = 0; e < E / 2; e++) row[e][b] = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
+                const int r = 2 * b + (k & 1) * 8 + (k >> 1);
+                if (!(have >> r & 1u)) continue;
+                float x[E];
                 uint32_t code[E];
                 __half2 meta[2];
-                quantise<D, G, false>(x[k], code, meta);
+                from_raw(raw[b % 2 * 2 + (k & 1) * 4 + (k >> 1)], x);
+                quantise<D, G, false>(x, code, meta);
 #pragma unroll
                 for (int e = 0; e < E / 2; e++) row[e][b] |= (code[2 * e] | code[2 * e + 1] << 4) << (8 * k);
                 if (lane * E % G == 0)
-                    *reinterpret_cast<__half2 *>(t + kv4_vmeta(D, G) +
-                                                 ((lane * E / G) * 16 + 2 * b + (k & 1) * 8 + (k >> 1)) * 4) = meta[0];
+                    *reinterpret_cast<__half2 *>(t + kv4_vmeta(D, G) + ((lane * E / G) * 16 + r) * 4) = meta[0];
+            }
+            const uint32_t four = 0x303u << (2 * b);
+            if ((have & four) != four) {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (have >> (2 * b + (k & 1) * 8 + (k >> 1)) & 1u)
+#pragma unroll
+                        for (int e = 0; e < E / 2; e++) codes[e * 16 + 4 * b + k] = static_cast<uint8_t>(row[e][b] >> (8 * k));
+            } else if (have != 0xffffu) {
+#pragma unroll
+                for (int e = 0; e < E / 2; e++) *reinterpret_cast<uint32_t *>(codes + e * 16 + 4 * b) = row[e][b];
             }
         }
+        if (have == 0xffffu) {
 #pragma unroll
-        for (int e = 0; e < E / 2; e++)
-            *reinterpret_cast<uint4 *>(t + kv4_val(D) + (lane * (E / 2) + e) * 16) =
-                make_uint4(row[e][0], row[e][1], row[e][2], row[e][3]);
-    }
-    for (uint32_t left = alone; left; left &= left - 1) {
-        const int64_t i = i0 + __ffs(left) - 1, slot = slot_of(i);
-        if (slot < 0) continue;
-        if (slot >= most) {
-            if (lane == 0) set_status(a.status, DEV_BAD_ARG);
-            continue;
+            for (int e = 0; e < E / 2; e++)
+                *reinterpret_cast<uint4 *>(codes + e * 16) = make_uint4(row[e][0], row[e][1], row[e][2], row[e][3]);
         }
-        float x[E];
-        uint32_t code[E];
-        __half2 meta[2];
-        load_head<T, D, false, VEC>(v + i * a.v_token, lane, x);
-        quantise<D, G, false>(x, code, meta);
-        write_codes<D, G, false>(tile_of(slot), static_cast<int>(slot % 16), lane, true, code, meta);
     }
 }
 
+// The values' warps come first: theirs is the most work each.
 template <typename T, int D, int G, bool SPLIT, int HEADS>
-__global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a, uint32_t token_warps) {
+__global__ void __launch_bounds__(128, 6) k_kv4_append(const AppendArgs a, uint32_t value_warps, uint32_t warps) {
     const uint32_t w = blockIdx.x * 4u + threadIdx.x / 32;
     const int lane = threadIdx.x & 31;
     grid_dep_wait();
-    if (w < token_warps) {
+    if (w < value_warps) {
         if (a.vec)
-            append_token<T, D, G, SPLIT, true, HEADS>(a, w, lane);
+            append_values<T, D, G, true>(a, w, lane);
         else
-            append_token<T, D, G, SPLIT, false, HEADS>(a, w, lane);
-    } else if (a.tiles && w - token_warps < (a.n + 15) / 16 * a.kv_heads) {
+            append_values<T, D, G, false>(a, w, lane);
+    } else if (w < warps) {
         if (a.vec)
-            append_values<T, D, G, true>(a, w - token_warps, lane);
+            append_token<T, D, G, SPLIT, true, HEADS>(a, w - value_warps, lane);
         else
-            append_values<T, D, G, false>(a, w - token_warps, lane);
+            append_token<T, D, G, SPLIT, false, HEADS>(a, w - value_warps, lane);
     }
 }
 
@@ -479,10 +489,12 @@ struct AppendLaunch {
     static st_status launch(st_handle *h, const AppendArgs &a) {
         const int64_t nk = (a.kv_heads + HEADS - 1) / HEADS, nq = a.q ? (a.heads + HEADS - 1) / HEADS : 0;
         const int64_t token_warps = a.n * (nq + nk + (a.tiles ? 0 : nk));
-        const int64_t warps = token_warps + (a.tiles ? (a.n + 15) / 16 * a.kv_heads : 0), blocks = (warps + 3) / 4;
+        const int64_t value_warps = a.tiles ? ((a.n + 15) / 16 + 1) * a.kv_heads : 0;
+        const int64_t warps = token_warps + value_warps, blocks = (warps + 3) / 4;
         if (warps > 0x7fffffff) return h->fail(ST_UNSUPPORTED_SHAPE, "st_kv4_append: too many tokens");
         ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_append<T, D, G, SPLIT, HEADS>, dim3(static_cast<unsigned>(blocks)),
-                                             dim3(128), 0, a, static_cast<uint32_t>(token_warps)));
+                                             dim3(128), 0, a, static_cast<uint32_t>(value_warps),
+                                             static_cast<uint32_t>(warps)));
         return st_after_launch(h, "k_kv4_append");
     }
 };
