@@ -85,8 +85,23 @@ __device__ __forceinline__ void store_head(T *out, int lane, const float (&x)[D 
     }
 }
 
+// Smallest and largest over the warp (sm_100's reduction of f32); NaN where one is.
+__device__ __forceinline__ void warp_range(float &lo, float &hi) {
+    asm("redux.sync.min.NaN.f32 %0, %0, 0xffffffff;" : "+f"(lo));
+    asm("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(hi));
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+}
+
 // Quantises a head by groups of G: the lane's codes, and for each of its
-// channels its group's {scale, zero}.
+// channels its group's {scale, zero}.  Only a group with a NaN or a value
+// outside the f16 range, which its extremes show, is looked through again.
 template <int D, int G, bool SPLIT>
 __device__ __forceinline__ void quantise(float (&x)[D / 32], uint32_t (&code)[D / 32], __half2 (&meta)[2]) {
     constexpr int E = D / 32;
@@ -94,17 +109,30 @@ __device__ __forceinline__ void quantise(float (&x)[D / 32], uint32_t (&code)[D 
     constexpr int LANES = G / PER < 32 ? G / PER : 32;             // lanes of a group
 #pragma unroll
     for (int set = 0; set < SETS; set++) {
-        float lo = 65504.0f, hi = -65504.0f;
+        const auto range = [&](float &lo, float &hi) {
+            lo = hi = x[set * PER];
 #pragma unroll
-        for (int e = set * PER; e < (set + 1) * PER; e++) {
-            x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
-        }
+            for (int e = set * PER + 1; e < (set + 1) * PER; e++) {
+                lo = min_nan(lo, x[e]);
+                hi = max_nan(hi, x[e]);
+            }
+            if constexpr (LANES == 32) {
+                warp_range(lo, hi);
+            } else {
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                for (int o = LANES / 2; o > 0; o >>= 1) {
+                    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                }
+            }
+        };
+        float lo, hi;
+        range(lo, hi);
+        if (__any_sync(0xffffffffu, !(lo >= -65504.0f && hi <= 65504.0f))) {
+#pragma unroll
+            for (int e = set * PER; e < (set + 1) * PER; e++)
+                x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+            range(lo, hi);
         }
         const __half zero = __float2half_rn(lo);
         const float z = __half2float(zero);
@@ -112,8 +140,11 @@ __device__ __forceinline__ void quantise(float (&x)[D / 32], uint32_t (&code)[D 
         const float s = __half2float(scale);
         const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
 #pragma unroll
-        for (int e = set * PER; e < (set + 1) * PER; e++)
-            code[e] = static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[e], z), inv)), 0.0f), 15.0f));
+        for (int e = set * PER; e < (set + 1) * PER; e++) {
+            // adding 1.5 2^23 rounds to a whole number, ties to even, in the sum's low bits
+            const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], z), inv), 0.0f), 15.0f);
+            code[e] = __float_as_uint(__fadd_rn(t, 12582912.0f)) & 15u;
+        }
         meta[set] = __halves2half2(scale, zero);
     }
     if (SETS == 1) meta[1] = meta[0];
@@ -276,6 +307,7 @@ __device__ __forceinline__ void append_token(const AppendArgs &a, uint32_t w, in
 template <typename T, int D, int G, bool VEC>
 __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, int lane) {
     constexpr int E = D / 32;
+    constexpr bool SPLIT = D == 128;  // groups of 64 lie in all lanes then; whole bytes in one lane either way
     const uint32_t sixteen = w / a.kv_heads;
     const int64_t i0 = sixteen * 16ll - 16, i = i0 + lane, most = a.n_pages * a.page;
     const int head = static_cast<int>(w - sixteen * a.kv_heads);
@@ -298,7 +330,7 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, i
         const T *src = v + (i0 + at) * a.v_token;
         const Place place(its * 16, a.page);
         uint8_t *t = a.data + ((place.page * a.kv_heads + head) * (a.page / 16) + place.off / 16) * kv4_tile_bytes(D, G);
-        uint8_t *codes = t + kv4_val(D) + lane * (E / 2) * 16;
+        const auto codes = [&](int e) { return t + kv4_val(D) + channel<D, SPLIT>(lane, 2 * e) / 2 * 16; };  // row of pair e
         uint32_t row[E / 2][4];
         Raw<T, D> raw[8];
 #pragma unroll
@@ -307,7 +339,7 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, i
 #pragma unroll
                 for (int k = 0; k < 8; k++)
                     if (have >> (2 * b + k % 4 + k / 4 * 8) & 1u)
-                        load_raw<T, D, false, VEC>(src + (2 * b + k % 4 + k / 4 * 8) * a.v_token, lane, raw[k]);
+                        load_raw<T, D, SPLIT, VEC>(src + (2 * b + k % 4 + k / 4 * 8) * a.v_token, lane, raw[k]);
             }
 #pragma unroll
             for (int e = 0; e < E / 2; e++) row[e][b] = 0;
@@ -319,11 +351,15 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, i
                 uint32_t code[E];
                 __half2 meta[2];
                 from_raw(raw[b % 2 * 2 + (k & 1) * 4 + (k >> 1)], x);
-                quantise<D, G, false>(x, code, meta);
+                quantise<D, G, SPLIT>(x, code, meta);
 #pragma unroll
                 for (int e = 0; e < E / 2; e++) row[e][b] |= (code[2 * e] | code[2 * e + 1] << 4) << (8 * k);
-                if (lane * E % G == 0)
-                    *reinterpret_cast<__half2 *>(t + kv4_vmeta(D, G) + ((lane * E / G) * 16 + r) * 4) = meta[0];
+#pragma unroll
+                for (int e = 0; e < E; e += SPLIT ? E / 2 : E) {
+                    const int c = channel<D, SPLIT>(lane, e);
+                    if (c % G == 0)
+                        *reinterpret_cast<__half2 *>(t + kv4_vmeta(D, G) + ((c / G) * 16 + r) * 4) = meta[e ? 1 : 0];
+                }
             }
             const uint32_t four = 0x303u << (2 * b);
             if ((have & four) != four) {
@@ -331,16 +367,16 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint32_t w, i
                 for (int k = 0; k < 4; k++)
                     if (have >> (2 * b + (k & 1) * 8 + (k >> 1)) & 1u)
 #pragma unroll
-                        for (int e = 0; e < E / 2; e++) codes[e * 16 + 4 * b + k] = static_cast<uint8_t>(row[e][b] >> (8 * k));
+                        for (int e = 0; e < E / 2; e++) codes(e)[4 * b + k] = static_cast<uint8_t>(row[e][b] >> (8 * k));
             } else if (have != 0xffffu) {
 #pragma unroll
-                for (int e = 0; e < E / 2; e++) *reinterpret_cast<uint32_t *>(codes + e * 16 + 4 * b) = row[e][b];
+                for (int e = 0; e < E / 2; e++) *reinterpret_cast<uint32_t *>(codes(e) + 4 * b) = row[e][b];
             }
         }
         if (have == 0xffffu) {
 #pragma unroll
             for (int e = 0; e < E / 2; e++)
-                *reinterpret_cast<uint4 *>(codes + e * 16) = make_uint4(row[e][0], row[e][1], row[e][2], row[e][3]);
+                *reinterpret_cast<uint4 *>(codes(e)) = make_uint4(row[e][0], row[e][1], row[e][2], row[e][3]);
         }
     }
 }
