@@ -118,10 +118,12 @@ SIGNATURES = {
     "st_knn_search_sharded": (_st, [_h, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
 }
 
+FUNCTIONS = {}
 for _name, (_res, _args) in SIGNATURES.items():
     _fn = getattr(lib, _name)
     _fn.restype = _res
     _fn.argtypes = _args
+    FUNCTIONS[_name] = _fn
 
 
 class StError(RuntimeError):

@@ -14,6 +14,7 @@ from . import _native as N
 
 _lock = threading.Lock()
 _handles = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's cudaStream_t, without a Stream object
 
 
 class Handle:
@@ -24,17 +25,19 @@ class Handle:
             stream = torch.cuda.current_stream(device).cuda_stream
             N.check(None, N.lib.st_create(device, ctypes.c_void_p(stream), ctypes.byref(h)))
         self.ptr = h
+        self.bound = stream
 
     def bind(self, stream=None):
         """Points the handle at `stream` (default: torch's current stream)."""
-        if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        N.lib.st_set_stream(self.ptr, ctypes.c_void_p(stream.cuda_stream))
+        raw = _raw_stream(self.device) if stream is None else stream.cuda_stream
+        if raw != self.bound:
+            N.lib.st_set_stream(self.ptr, raw)
+            self.bound = raw
         return self.ptr
 
     def call(self, name, *args):
-        fn = getattr(N.lib, name)
-        return N.check(self.ptr, fn(self.bind(), *args))
+        status = N.FUNCTIONS[name](self.bind(), *args)
+        return status if status == N.ST_OK else N.check(self.ptr, status)
 
     def sync(self):
         return N.check(self.ptr, N.lib.st_sync(self.bind()))
@@ -54,6 +57,9 @@ class Handle:
 
 def handle(device=None):
     """The handle of `device` (default: torch's current CUDA device)."""
+    h = _handles.get(device.index if isinstance(device, torch.device) else device)
+    if h is not None:
+        return h
     if not torch.cuda.is_available():
         raise RuntimeError("scratchtape_b200 needs a CUDA device (sm_100a); none is visible")
     if device is None:

@@ -15,11 +15,12 @@ slot or a page number out of range) is reported by ``handle().sync()``.  There
 is no counterpart in the reference, whose sequences always run whole.
 """
 import ctypes
+import functools
 
 import torch
 
 from . import _native as N
-from .device import handle, ptr
+from .device import handle
 
 _DTYPES = {torch.float32: N.ST_F32, torch.float16: N.ST_F16, torch.bfloat16: N.ST_BF16}
 
@@ -38,28 +39,36 @@ def empty(pages: int, page: int, kv_heads: int, d: int, group: int = 64, device=
 
 
 def _cache(data: torch.Tensor, d: int, group: int):
-    if data.dtype != torch.uint8 or data.dim() != 4 or not data.is_contiguous() or not data.is_cuda:
+    if data.dtype is not torch.uint8 or data.dim() != 4 or not data.is_cuda or not data.is_contiguous():
         raise ValueError("the cache is a contiguous uint8 CUDA tensor [pages, kv_heads, page / 16, tile]")
-    if group < 1 or d % group or data.shape[3] != tile_bytes(d, group):
-        raise ValueError("tiles of %d bytes do not hold heads of %d in groups of %d" % (data.shape[3], d, group))
-    return data.shape[0], data.shape[2] * 16, data.shape[1]
+    pages, kv_heads, tiles, tile = data.shape
+    if group < 1 or d % group or tile != 16 * d + 128 * (d // group):
+        raise ValueError("tiles of %d bytes do not hold heads of %d in groups of %d" % (tile, d, group))
+    return pages, tiles * 16, kv_heads, data.device
 
 
-def _whole(t: torch.Tensor, dtype, like: torch.Tensor, name: str, shape=None):
-    if t.dtype != dtype or not t.is_contiguous() or t.device != like.device:
-        raise ValueError("%s must be a contiguous %s tensor on %s" % (name, str(dtype)[6:], like.device))
-    if shape is not None and tuple(t.shape) != tuple(shape):
+def _whole(t: torch.Tensor, dtype, device, name: str, shape=None):
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous %s tensor on %s" % (name, str(dtype)[6:], device))
+    if shape is not None and t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
     return t
 
 
-def _rows(t: torch.Tensor, dtype, like: torch.Tensor, name: str, shape):
+def _rows(t: torch.Tensor, dtype, device, name: str, shape):
     """t [n, heads, d] with contiguous rows of d (any strides between them)."""
-    if t.dtype != dtype or t.device != like.device:
-        raise ValueError("%s must be a %s tensor on %s" % (name, str(dtype)[6:], like.device))
-    if tuple(t.shape) != tuple(shape):
+    if t.dtype is not dtype or t.device != device:
+        raise ValueError("%s must be a %s tensor on %s" % (name, str(dtype)[6:], device))
+    if t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
     return t if t.stride(2) == 1 else t.contiguous()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(device, *shapes):
+    need = ctypes.c_int64()
+    handle(device).call("st_kv4_attn_workspace", *shapes, ctypes.byref(need))
+    return need.value
 
 
 def append(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, group: int = 64, q=None,
@@ -67,47 +76,57 @@ def append(data: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     """Writes tokens k, v [n, kv_heads, d] (float32, float16 or bfloat16) to ``slots`` (int64 [n], all different;
     negative: left out).  With cos and sin (float32 [positions, rotary / 2]) and ``positions`` (int32 [n]) the first
     ``rotary`` channels of the keys are rotated first, and those of q [n, heads, d], which is returned (into ``out``)."""
-    n, kv_heads, d = k.shape
-    pages, page, have = _cache(data, d, group)
+    n, _, d = k.shape
+    pages, page, kv_heads, device = _cache(data, d, group)
     dtype = k.dtype
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError("keys in %s" % dtype)
-    k = _rows(k, dtype, data, "k", (n, have, d))
-    v = _rows(v, dtype, data, "v", (n, have, d))
-    _whole(slots, torch.int64, data, "slots", (n,))
-    rotary, table, heads, qs = 0, 0, 0, (0, 0)
+    k = _rows(k, dtype, device, "k", (n, kv_heads, d))
+    v = _rows(v, dtype, device, "v", (n, kv_heads, d))
+    _whole(slots, torch.int64, device, "slots", (n,))
+    rotary = table = heads = q_token = q_head = 0
+    q_ptr = out_ptr = cos_ptr = sin_ptr = pos_ptr = None
     if cos is not None:
-        table, rotary = cos.shape[0], 2 * cos.shape[1]
-        _whole(cos, torch.float32, data, "cos"), _whole(sin, torch.float32, data, "sin", cos.shape)
-        _whole(positions, torch.int32, data, "positions", (n,))
+        _whole(cos, torch.float32, device, "cos")
+        _whole(sin, torch.float32, device, "sin", cos.shape)
+        table, rotary = cos.shape
+        rotary *= 2
+        if rotary:
+            _whole(positions, torch.int32, device, "positions", (n,))
+            cos_ptr, sin_ptr, pos_ptr = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
     if q is not None:
-        if cos is None:
+        if not rotary:
             raise ValueError("queries are only rotated: without cos and sin there is nothing to do")
         heads = q.shape[1]
-        q = _rows(q, dtype, data, "q", (n, heads, d))
-        qs = q.stride()
-        out = torch.empty((n, heads, d), dtype=dtype, device=q.device) if out is None else \
-            _whole(out, dtype, data, "out", (n, heads, d))
-    handle(data.device).call("st_kv4_append", ptr(data), pages, page, kv_heads, d, group, ptr(k), k.stride(0),
-                             k.stride(1), ptr(v), v.stride(0), v.stride(1), ptr(slots), n, ptr(q), qs[0], qs[1],
-                             ptr(out) if q is not None else None, heads, ptr(cos), ptr(sin),
-                             ptr(positions) if rotary else None, table, rotary, int(interleaved), _DTYPES[dtype])
+        q = _rows(q, dtype, device, "q", (n, heads, d))
+        out = torch.empty((n, heads, d), dtype=dtype, device=device) if out is None else \
+            _whole(out, dtype, device, "out", (n, heads, d))
+        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+        q_token, q_head, _ = q.stride()
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    handle(device).call("st_kv4_append", data.data_ptr(), pages, page, kv_heads, d, group, k.data_ptr(), k_token, k_head,
+                        v.data_ptr(), v_token, v_head, slots.data_ptr(), n, q_ptr, q_token, q_head, out_ptr, heads,
+                        cos_ptr, sin_ptr, pos_ptr, table, rotary, interleaved, code)
     return out if q is not None else None
 
 
 def read(data: torch.Tensor, slots: torch.Tensor, d: int, group: int = 64, dtype=torch.float32, out=None):
     """-> (k, v) [n, kv_heads, d]: what the cache holds in ``slots`` (int64 [n]; negative: zeros)."""
-    pages, page, kv_heads = _cache(data, d, group)
-    if dtype not in _DTYPES:
+    pages, page, kv_heads, device = _cache(data, d, group)
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError("values in %s" % dtype)
-    _whole(slots, torch.int64, data, "slots", slots.shape[:1])
-    shape = (slots.shape[0], kv_heads, d)
+    n = slots.shape[0]
+    _whole(slots, torch.int64, device, "slots", (n,))
+    shape = (n, kv_heads, d)
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=data.device), torch.empty(shape, dtype=dtype,
-                                                                                device=data.device))
-    _whole(out[0], dtype, data, "out[0]", shape), _whole(out[1], dtype, data, "out[1]", shape)
-    handle(data.device).call("st_kv4_read", ptr(data), pages, page, kv_heads, d, group, ptr(slots), shape[0],
-                             ptr(out[0]), ptr(out[1]), _DTYPES[dtype])
+        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _whole(out[0], dtype, device, "out[0]", shape), _whole(out[1], dtype, device, "out[1]", shape)
+    handle(device).call("st_kv4_read", data.data_ptr(), pages, page, kv_heads, d, group, slots.data_ptr(), n,
+                        out[0].data_ptr(), out[1].data_ptr(), code)
     return out
 
 
@@ -121,18 +140,21 @@ def attend(q: torch.Tensor, data: torch.Tensor, pages: torch.Tensor, kv_len: tor
     lie in pages[b] (int32 [batch, most]).  ``causal``: a row sees the keys up to its own position; ``window``: only
     the last ``window`` of them; ``one``: softmax1.  A row that sees nothing gives 0 (lse -inf; softmax1: 0)."""
     rows, heads, d = q.shape
-    n_pages, page, kv_heads = _cache(data, d, group)
+    n_pages, page, kv_heads, device = _cache(data, d, group)
     dtype = q.dtype
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError("queries in %s" % dtype)
     if heads % kv_heads:
         raise ValueError("%d heads do not share %d" % (heads, kv_heads))
-    q = _rows(q, dtype, data, "q", (rows, heads, d))
+    q = _rows(q, dtype, device, "q", (rows, heads, d))
     batch = kv_len.shape[0]
-    _whole(kv_len, torch.int32, data, "kv_len", (batch,))
-    _whole(pages, torch.int32, data, "pages", (batch, pages.shape[-1]))
+    _whole(kv_len, torch.int32, device, "kv_len", (batch,))
+    most = pages.shape[-1]
+    _whole(pages, torch.int32, device, "pages", (batch, most))
+    start_ptr = None
     if q_start is not None:
-        _whole(q_start, torch.int32, data, "q_start", (batch + 1,))
+        start_ptr = _whole(q_start, torch.int32, device, "q_start", (batch + 1,)).data_ptr()
         max_q = rows if max_q is None else max_q
     elif rows != batch:
         raise ValueError("%d rows for %d sequences: q_start says whose they are" % (rows, batch))
@@ -140,16 +162,16 @@ def attend(q: torch.Tensor, data: torch.Tensor, pages: torch.Tensor, kv_len: tor
         max_q = 1
     if window < 0 or (rows and max_q < 1):
         raise ValueError("window %d, max_q %d" % (window, max_q))
-    o = torch.empty((rows, heads, d), dtype=dtype, device=q.device) if out is None else \
-        _whole(out, dtype, data, "out", (rows, heads, d))
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    o = torch.empty((rows, heads, d), dtype=dtype, device=device) if out is None else \
+        _whole(out, dtype, device, "out", (rows, heads, d))
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=device) if return_lse else None
     if rows and batch:
-        h = handle(data.device)
-        need = ctypes.c_int64()
-        h.call("st_kv4_attn_workspace", batch, rows, max_q, pages.shape[1] * page, heads, kv_heads, d, ctypes.byref(need))
         # torch's allocator gives each stream, and each captured graph, a workspace of its own
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        h.call("st_kv4_attn", ptr(q), q.stride(0), q.stride(1), ptr(o), ptr(lse), ptr(data), n_pages, page, heads,
-               kv_heads, d, group, ptr(pages), pages.shape[1], ptr(kv_len), ptr(q_start), batch, rows, max_q,
-               float(scale), int(causal), int(one), window, _DTYPES[dtype], ptr(work), need.value)
+        need = _workspace(device, batch, rows, max_q, most * page, heads, kv_heads, d)
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+        q_token, q_head, _ = q.stride()
+        handle(device).call("st_kv4_attn", q.data_ptr(), q_token, q_head, o.data_ptr(),
+                            lse.data_ptr() if return_lse else None, data.data_ptr(), n_pages, page, heads, kv_heads, d,
+                            group, pages.data_ptr(), most, kv_len.data_ptr(), start_ptr, batch, rows, max_q, scale,
+                            causal, one, window, code, work.data_ptr(), need)
     return (o, lse) if return_lse else o
