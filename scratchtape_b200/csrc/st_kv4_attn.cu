@@ -17,84 +17,18 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "st_kv4.cuh"
+#include "st_kv4_attn.cuh"
+#include "st_kv4_tiles.cuh"
 
 namespace {
 
 using namespace st;
 
-struct AttnArgs {
-    const void *q;
-    int64_t q_token, q_head;
-    void *o;
-    float *lse;
-    const uint8_t *data;
-    int64_t n_pages;
-    int page, heads, kv_heads, share;
-    const int32_t *pages;
-    int64_t max_pages;
-    const int32_t *kv_len, *q_start;
-    int64_t batch, rows;
-    int max_q;
-    uint32_t page_magic;  // ceil(2^32 / (page / 16)), 0 for pages of one tile
-    float scale_log2;  // scale * log2(e): scores are kept in units of log 2
-    int causal, one, window;
-    int vec;           // rows of q start on 16-byte boundaries
-    int sms, parts;    // parts at most
-    int item_blocks;   // blocks of rows of a sequence at most, where notes go by item; else 0
-    int64_t notes;     // notes at the start of the workspace
-    float *work;       // notes, then the pieces' partial results
-    int *status;
-};
-
 // ---- which keys a sequence's rows see, and how the work is cut ---------------
 
-constexpr int UNIT = 32;     // keys of one step of a warp: two tiles
 constexpr int WARPS = 4;     // warps of a block; they take a piece's units in turn
 constexpr int PAD = 8;       // what starting a piece costs, in units of a team's work
 constexpr int MIN_PART = 4 + PAD;  // of a part at least: a unit for each warp
-
-struct Seq {
-    int64_t first;         // its first row
-    int count, len;        // rows, keys
-    int u0, units, blocks;  // units from u0 (at least one, where it has rows); blocks of RB rows of each head
-};
-
-// Sequence b, with lengths that do not fit left out (and reported).
-template <int RB>
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t b) {
-    Seq s;
-    s.first = b;
-    s.count = 1;
-    bool bad = false;
-    if (a.q_start) {
-        const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
-        s.first = q0;
-        s.count = q1 - q0;
-        if (q0 < 0 || q1 < q0 || q1 > a.rows || s.count > a.max_q) {
-            s.count = 0;
-            bad = true;
-        }
-    }
-    s.len = a.kv_len[b];
-    const int most = static_cast<int>(a.max_pages * a.page);
-    if (s.len < 0 || s.len > most) {
-        s.len = s.len < 0 ? 0 : most;
-        bad = true;
-    }
-    if (bad) set_status(a.status, DEV_BAD_ARG);
-    const int begin = a.window > 0 ? max(0, s.len - s.count + 1 - a.window) : 0;
-    s.u0 = begin / UNIT;
-    s.units = max(1, (s.len + UNIT - 1) / UNIT - s.u0);
-    s.blocks = (s.count * a.share + RB - 1) / RB;
-    return s;
-}
-
-// Keys [x, y) that row r of (query, shared head) of sequence s sees.
-__device__ __forceinline__ int2 seen_by(const AttnArgs &a, const Seq &s, int r) {
-    const int pos = s.len - s.count + min(r, s.count * a.share - 1) / a.share;
-    return make_int2(a.window > 0 ? max(0, pos - a.window + 1) : 0, a.causal ? min(s.len, pos + 1) : s.len);
-}
 
 template <int RB>
 __device__ __forceinline__ int64_t weight_of(const AttnArgs &a, int64_t b) {
@@ -209,19 +143,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack2(uint32_t x) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&x));
-}
-
 // Words of a thread's part of a group's row of key codes: G / 32 of 32 bits.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
@@ -233,32 +154,6 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
     } else {
         const uint4 x = *reinterpret_cast<const uint4 *>(p);
         w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, int vec, float (&x)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                T e[2];
-                memcpy(e, &w[i], 4);
-                x[2 * i] = to_f32(e[0]);
-                x[2 * i + 1] = to_f32(e[1]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float4 v = reinterpret_cast<const float4 *>(p)[i];
-                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
     }
 }
 
@@ -867,8 +762,27 @@ st_status launch(st_handle *h, AttnArgs a) {
     return st_after_launch(h, "k_kv4_attn_join");
 }
 
+// Many rows of 16-bit types go by tiles of 128 (a positive scale: the largest
+// score is the largest product).
+bool by_tiles(const AttnArgs &a, int dtype) {
+    return dtype != ST_F32 && a.scale_log2 > 0.0f && a.max_q * static_cast<int64_t>(a.share) >= 32 && a.batch <= 65535;
+}
+
+template <typename T, int D, int G>
+st_status launch_tiles(st_handle *h, const AttnArgs &a) {
+    using L = Tiles<T, D, G>;
+    const int64_t blocks = (a.max_q * static_cast<int64_t>(a.share) + L::ROWS - 1) / L::ROWS;
+    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_kv4_attn_tiles<T, D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SIZE));
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn_tiles<T, D, G>,
+                                         dim3(static_cast<unsigned>(blocks), a.kv_heads, static_cast<unsigned>(a.batch)),
+                                         dim3(L::THREADS), L::SIZE, a));
+    return st_after_launch(h, "k_kv4_attn_tiles");
+}
+
 template <typename T, int D, int G>
 st_status by_columns(st_handle *h, const AttnArgs &a, int nt) {
+    if constexpr (sizeof(T) == 2)
+        if (by_tiles(a, std::is_same<T, __half>::value ? ST_F16 : ST_BF16)) return launch_tiles<T, D, G>(h, a);
     return nt == 1 ? launch<T, D, G, 1>(h, a) : launch<T, D, G, 2>(h, a);
 }
 

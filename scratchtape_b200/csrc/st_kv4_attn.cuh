@@ -1,0 +1,114 @@
+// st_kv4_attn.cuh -- what the kernels of attention over the 4-bit cache share:
+// their arguments, which keys a row sees, conversions.
+#pragma once
+#include "st_kv4.cuh"
+
+namespace st {
+
+struct AttnArgs {
+    const void *q;
+    int64_t q_token, q_head;
+    void *o;
+    float *lse;
+    const uint8_t *data;
+    int64_t n_pages;
+    int page, heads, kv_heads, share;
+    const int32_t *pages;
+    int64_t max_pages;
+    const int32_t *kv_len, *q_start;
+    int64_t batch, rows;
+    int max_q;
+    uint32_t page_magic;  // ceil(2^32 / (page / 16)), 0 for pages of one tile
+    float scale_log2;  // scale * log2(e): scores are kept in units of log 2
+    int causal, one, window;
+    int vec;           // rows of q start on 16-byte boundaries
+    int sms, parts;    // parts at most
+    int item_blocks;   // blocks of rows of a sequence at most, where notes go by item; else 0
+    int64_t notes;     // notes at the start of the workspace
+    float *work;       // notes, then the pieces' partial results
+    int *status;
+};
+
+constexpr int UNIT = 32;     // keys of one step of a warp: two tiles
+struct Seq {
+    int64_t first;         // its first row
+    int count, len;        // rows, keys
+    int u0, units, blocks;  // units from u0 (at least one, where it has rows); blocks of RB rows of each head
+};
+
+// Sequence b, with lengths that do not fit left out (and reported).
+template <int RB>
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int64_t b) {
+    Seq s;
+    s.first = b;
+    s.count = 1;
+    bool bad = false;
+    if (a.q_start) {
+        const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
+        s.first = q0;
+        s.count = q1 - q0;
+        if (q0 < 0 || q1 < q0 || q1 > a.rows || s.count > a.max_q) {
+            s.count = 0;
+            bad = true;
+        }
+    }
+    s.len = a.kv_len[b];
+    const int most = static_cast<int>(a.max_pages * a.page);
+    if (s.len < 0 || s.len > most) {
+        s.len = s.len < 0 ? 0 : most;
+        bad = true;
+    }
+    if (bad) set_status(a.status, DEV_BAD_ARG);
+    const int begin = a.window > 0 ? max(0, s.len - s.count + 1 - a.window) : 0;
+    s.u0 = begin / UNIT;
+    s.units = max(1, (s.len + UNIT - 1) / UNIT - s.u0);
+    s.blocks = (s.count * a.share + RB - 1) / RB;
+    return s;
+}
+
+// Keys [x, y) that row r of (query, shared head) of sequence s sees.
+__device__ __forceinline__ int2 seen_by(const AttnArgs &a, const Seq &s, int r) {
+    const int pos = s.len - s.count + min(r, s.count * a.share - 1) / a.share;
+    return make_int2(a.window > 0 ? max(0, pos - a.window + 1) : 0, a.causal ? min(s.len, pos + 1) : s.len);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int vec, float (&x)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                T e[2];
+                memcpy(e, &w[i], 4);
+                x[2 * i] = to_f32(e[0]);
+                x[2 * i + 1] = to_f32(e[1]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float4 v = reinterpret_cast<const float4 *>(p)[i];
+                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+    }
+}
+
+}  // namespace st

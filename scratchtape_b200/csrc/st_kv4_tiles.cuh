@@ -1,0 +1,379 @@
+// st_kv4_tiles.cuh -- attention of many rows over the 4-bit cache on tcgen05.
+//
+// Pieces of prompts have hundreds of rows for each kv head, and the products,
+// not the cache's bytes, bound them: 4 d flop for each row and key it sees.  One block
+// takes 128 rows of (query, shared head) and goes over its keys 64 at a time.
+// Four warps turn codes into f16 operands in swizzled shared memory (keys as
+// they lie, values transposed by descriptor), one thread issues the
+// products, and four warps, a thread a row, take the scores from TMEM to
+// weights and put them back into the same TMEM columns as the A operand of the
+// second product.  Two blocks share an SM, so one's products run while the
+// other's softmax does (the exponentials take about as long as the products:
+// 64 x 128 of them at 16 a clock against 2 x 128 x 64 x d multiplies).
+//
+// Roundings: queries are exact in f16 (a power of two per row), c * scale +
+// zero is rounded to f16 once (2^-12 of a key or value), weights to f16.
+#pragma once
+#include "st_kv4_attn.cuh"
+
+namespace st {
+
+// Channels of an operand lie in the order 0 4 1 5 2 6 3 7 of every eight: the
+// order in which masks take a word's nibbles.  Queries are put in it too, and
+// results come out of it.
+__device__ __forceinline__ constexpr int kv4_lane_of(int e) { return (e & 3) * 2 + (e >> 2); }
+
+// Eight codes of a word times scale plus zero, in that order.
+__device__ __forceinline__ uint4 kv4_expand(uint32_t w, __half2 s, __half2 z) {
+    const __half2 low = __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x6400));      // 1024
+    const __half2 sixteenth = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));  // 1 / 16
+    const __half2 down = __halves2half2(__ushort_as_half(0xd400), __ushort_as_half(0xd400));     // -64
+    uint32_t out[4];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t v = w >> (8 * k), a = (v & 0x000f000fu) | 0x64006400u, b = (v & 0x00f000f0u) | 0x64006400u;
+        // 1024 + c less 1024, and (1024 + 16 c) / 16 less 64: the codes, exactly
+        const __half2 x = __hfma2(__hsub2(*reinterpret_cast<const __half2 *>(&a), low), s, z);
+        const __half2 y = __hfma2(__hfma2(*reinterpret_cast<const __half2 *>(&b), sixteenth, down), s, z);
+        out[2 * k] = *reinterpret_cast<const uint32_t *>(&x);
+        out[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&y);
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+template <typename T, int D, int G>
+struct Tiles {
+    static constexpr int ROWS = 128, KEYS = 64, CHUNKS = D / 64;
+    static constexpr int Q = 0, K = Q + CHUNKS * ROWS * 128, KBYTES = CHUNKS * KEYS * 128;
+    static constexpr int V = K + 2 * KBYTES, BAR = V + 2 * KBYTES, SIZE = BAR + 256 + 1024;
+    static constexpr int THREADS = 288;
+    static constexpr uint32_t TMEM = 256;  // O (d columns), two score tiles (64 each)
+};
+
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
+    using L = Tiles<T, D, G>;
+    constexpr int ROWS = L::ROWS, KEYS = L::KEYS, NG = D / G, TILE = kv4_tile_bytes(D, G);
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::BAR);
+    uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8, *p_full = bar + 10,
+             *o_done = bar + 12, *q_full = bar + 13;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 14), *oks = tslot + 4;  // oks[4]: tiles that are there, by block % 4
+    const int tid = threadIdx.x, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&k_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+        }
+        mbar_init(o_done, 1);
+        mbar_init(q_full, 128);
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(tslot, L::TMEM);
+        tmem_relinquish();
+    }
+    grid_dep_wait();
+    grid_dep_launch();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tslot, t_o = tmem, t_s = tmem + D;
+    const int head = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const Seq s = seq_of<ROWS>(a, b);
+    const int row0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * ROWS;  // most keys first
+    const int n_rows = s.count * a.share;
+    int first = 0, n = 0;  // blocks of keys
+    int2 all = make_int2(0, 0);
+    if (row0 < n_rows) {
+        const int2 top = seen_by(a, s, row0), last = seen_by(a, s, row0 + ROWS - 1);
+        all = make_int2(last.x, top.y);  // what every row sees
+        first = top.x / KEYS;
+        n = max(0, (last.y + KEYS - 1) / KEYS - first);
+    }
+    bool dead = false;
+    const auto wait = [&](uint64_t *x, int parity) {  // once one has run out, none is waited for
+        if (!dead) dead = !mbar_wait(x, parity, a.status, DEV_TIMEOUT_FULL);
+    };
+
+    if (warp < 4) {
+        const int r = row0 + tid;
+        const bool real = r < n_rows;
+        const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+        float c1 = 0.0f;
+        {
+            const T *q = static_cast<const T *>(a.q);
+            if (real)
+                q += (s.first + r / a.share) * a.q_token + (static_cast<int64_t>(head) * a.share + r % a.share) * a.q_head;
+            float top = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; c++) {
+                float x[8] = {};
+                if (real) load8(q + 8 * c, a.vec, x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+            }
+            const int top_exp = static_cast<int>(__float_as_uint(top) >> 23);
+            const int up = top_exp > 0 ? max(-100, min(100, 14 + 127 - top_exp)) : 0;
+            // products with keys of the f16 range stay far inside f32's
+            const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+            c1 = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * a.scale_log2;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; c++) {
+                float x[8] = {};
+                if (real) load8(q + 8 * c, a.vec, x);
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] = pack2(x[k] * mul, x[k + 4] * mul);
+                *reinterpret_cast<uint4 *>(smem + L::Q + c / 8 * (ROWS * 128) + sw128_offset(tid, c % 8)) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+        const int2 sees = real ? seen_by(a, s, r) : make_int2(0, 0);
+        float ref = 0.0f, l = 0.0f;
+        bool seen = false;
+        for (int j = 0; j < n; j++) {
+            const int st = j & 1, key0 = (first + j) * KEYS;
+            wait(&s_full[st], j >> 1 & 1);
+            tc_fence_after();
+            uint32_t x[KEYS];
+            tmem_ld32(t_s + lane_base + st * KEYS, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+            tmem_ld32(t_s + lane_base + st * KEYS + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+            tmem_ld_wait();
+            const uint32_t there = oks[j & 3];
+            if (key0 < all.x || key0 + KEYS > all.y || there != 15u) {
+                asm volatile("");
+#pragma unroll
+                for (int i = 0; i < KEYS; i++)
+                    if (key0 + i < sees.x || key0 + i >= sees.y || !(there >> (i / 16) & 1u)) x[i] = 0xff800000u;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < KEYS; i++) top = fmaxf(top, __uint_as_float(x[i]));
+            top *= c1;  // c1 > 0
+            const bool move = top > -INFINITY && (!seen || top > ref + 8.0f);
+            if (__any_sync(0xffffffffu, move)) {
+                const float fix = move && seen ? exp2_fast(ref - top) : 1.0f;
+                if (move) {
+                    ref = top;
+                    seen = true;
+                    l *= fix;
+                }
+                if (j > 0) {
+                    wait(o_done, (j - 1) & 1);  // the product before has been added
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + lane_base + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                        tmem_st32(t_o + lane_base + c, o);
+                    }
+                }
+            }
+            uint32_t p[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const float u = exp2_fast(fmaf(__uint_as_float(x[2 * i]), c1, -ref)),
+                            v = exp2_fast(fmaf(__uint_as_float(x[2 * i + 1]), c1, -ref));
+                l += u + v;
+                p[i] = pack2(u, v);
+            }
+            tmem_st32(t_s + lane_base + st * KEYS, p);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[st]);
+        }
+        if (n > 0) wait(o_done, (n - 1) & 1);
+        tc_fence_after();
+        float top = ref, sum = l, fix = 1.0f;
+        if (a.one) {
+            top = seen ? fmaxf(ref, 0.0f) : 0.0f;
+            fix = seen ? exp2_fast(ref - top) : 0.0f;
+            sum = l * fix + exp2_fast(-top);
+        }
+        const float inv = sum > 0.0f || sum != sum ? fix / sum : 0.0f;
+        const int64_t out = real ? (s.first + r / a.share) * a.heads + static_cast<int64_t>(head) * a.share + r % a.share : 0;
+        T *dst = static_cast<T *>(a.o) + out * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            if (n > 0) {
+                tmem_ld32(t_o + lane_base + c, o);
+                tmem_ld_wait();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = 0;
+            }
+            if (!real) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+                T y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = from_f32<T>(seen ? __uint_as_float(o[i + kv4_lane_of(e)]) * inv : 0.0f);
+                uint4 v;
+                memcpy(&v, y, 16);
+                *reinterpret_cast<uint4 *>(dst + c + i) = v;
+            }
+        }
+        if (real && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+    } else if (warp < 8) {
+        const int t = tid - 128;
+        const int32_t *table = a.pages + b * a.max_pages;
+        const int n_tiles = (s.len + 15) / 16, page_tiles = a.page / 16;
+        // keys: key t % 64, the half t / 64 of its channels
+        constexpr int HALF = D / 2, KWORDS = HALF / 8, KG = HALF < G ? 1 : HALF / G;
+        const int key = t & 63, c0 = (t >> 6) * HALF;
+        // values: the octet of channels and the words (four tokens each) of a tile's rows
+        constexpr int OCT = D / 8, WORDS = D == 128 ? 2 : 1;
+        const int oct = t % OCT, part = t / OCT, v_tile = part / (4 / WORDS), j0 = part % (4 / WORDS) * WORDS;
+        const auto page_of = [&](int tile) { return tile < n_tiles ? table[a.page_magic ? __umulhi(tile, a.page_magic) : tile] : -1; };
+        const auto at = [&](int tile, int page) -> const uint8_t * {
+            if (tile >= n_tiles || page < 0 || page >= a.n_pages) return nullptr;
+            const int in = tile - (a.page_magic ? __umulhi(tile, a.page_magic) : tile) * page_tiles;
+            return a.data + ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + in) * TILE;
+        };
+        uint32_t kw[KWORDS], vw[4][WORDS];
+        __half2 km[KG], vm[WORDS][4];
+        uint32_t there = 0;
+        int k_page = -1, v_page = -1, lane_page = -1;
+        const auto pages = [&](int j) {  // of block j
+            const int tile = (first + j) * 4;
+            k_page = page_of(tile + key / 16);
+            v_page = page_of(tile + v_tile);
+            lane_page = page_of(tile + (t & 3));
+        };
+        const auto load = [&](int j) {  // block j's codes to registers
+            const int tile = (first + j) * 4, k_tile = tile + key / 16;
+            const uint8_t *p = at(k_tile, k_page), *q = at(tile + v_tile, v_page);
+            const int r = key & 15;
+            const bool here = p && k_tile * 16 + r < s.len;
+#pragma unroll
+            for (int i = 0; i < KWORDS; i++) kw[i] = 0;
+#pragma unroll
+            for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
+            if (here) {
+                constexpr int PER = KWORDS / KG;
+#pragma unroll
+                for (int g = 0; g < KG; g++) {
+                    const int c = c0 + g * (HALF / KG);
+                    const uint8_t *src = p + (c / G) * 8 * G + r * (G / 2) + (c % G) / 2;
+#pragma unroll
+                    for (int i = 0; i < PER; i += 4) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(src + 4 * i);
+                        kw[g * PER + i] = v.x, kw[g * PER + i + 1] = v.y, kw[g * PER + i + 2] = v.z, kw[g * PER + i + 3] = v.w;
+                    }
+                    km[g] = reinterpret_cast<const __half2 *>(p + kv4_kmeta(D))[(c / G) * 16 + r];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int w = 0; w < WORDS; w++)
+                    vw[i][w] = q ? *reinterpret_cast<const uint32_t *>(q + kv4_val(D) + (oct * 4 + i) * 16 + 4 * (j0 + w)) : 0;
+#pragma unroll
+            for (int w = 0; w < WORDS; w++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int token = 2 * (j0 + w) + (k & 1) * 8 + (k >> 1);
+                    const bool real = q && (tile + v_tile) * 16 + token < s.len;
+                    vm[w][k] = real ? reinterpret_cast<const __half2 *>(q + kv4_vmeta(D, G))[(oct * 8 / G) * 16 + token]
+                                    : __floats2half2_rn(0.0f, 0.0f);
+                }
+            const bool ok = lane_page >= 0 && lane_page < a.n_pages;
+            if (t < 4 && tile + t < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
+            there = __ballot_sync(0xffffffffu, ok || tile + (t & 3) >= n_tiles) & 15u;
+        };
+        if (n > 0) {
+            pages(0);
+            load(0);
+            if (n > 1) pages(1);
+        }
+        for (int j = 0; j < n; j++) {
+            const int st = j & 1;
+            uint8_t *ks = smem + L::K + st * L::KBYTES, *vs = smem + L::V + st * L::KBYTES;
+            if (j >= 2) wait(&k_empty[st], (j >> 1) - 1 & 1);
+            if (t == 0) oks[j & 3] = there;
+#pragma unroll
+            for (int i = 0; i < KWORDS; i++) {
+                const __half2 m = km[i / (KWORDS / KG)];
+                const int c = c0 / 8 + i;
+                *reinterpret_cast<uint4 *>(ks + c / 8 * (KEYS * 128) + sw128_offset(key, c % 8)) =
+                    kv4_expand(kw[i], __low2half2(m), __high2half2(m));
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&k_full[st]);
+            if (j >= 2) wait(&v_empty[st], (j >> 1) - 1 & 1);
+#pragma unroll
+            for (int w = 0; w < WORDS; w++) {
+                // four pairs' bytes of four tokens -> four tokens' eight channels
+                const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), x1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+                const uint32_t y0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+                const uint32_t tok[4] = {__byte_perm(x0, y0, 0x5410), __byte_perm(x0, y0, 0x7632),
+                                         __byte_perm(x1, y1, 0x5410), __byte_perm(x1, y1, 0x7632)};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int row = v_tile * 16 + 2 * (j0 + w) + (k & 1) * 8 + (k >> 1);
+                    *reinterpret_cast<uint4 *>(vs + oct / 8 * (KEYS * 128) + sw128_offset(row, oct % 8)) =
+                        kv4_expand(tok[k], __low2half2(vm[w][k]), __high2half2(vm[w][k]));
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&v_full[st]);
+            if (j + 1 < n) {
+                load(j + 1);
+                if (j + 2 < n) pages(j + 2);
+            }
+        }
+    } else if (tid == 256 && n > 0) {
+        const uint32_t qa = smem_u32(smem + L::Q), ka = smem_u32(smem + L::K), va = smem_u32(smem + L::V);
+        constexpr uint32_t id_s = idesc_make(1, 0, false, false, ROWS, KEYS), id_o = idesc_make(1, 0, false, true, ROWS, D);
+        const auto scores = [&](int j) {
+            const int st = j & 1;
+            wait(&k_full[st], j >> 1 & 1);
+            tc_fence_after();
+            if (!dead)
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++)
+                    umma_f16(t_s + st * KEYS, sdesc_sw128(qa + (kk >> 2) * (ROWS * 128) + (kk & 3) * 32, 16, 1024),
+                             sdesc_sw128(ka + st * L::KBYTES + (kk >> 2) * (KEYS * 128) + (kk & 3) * 32, 16, 1024), id_s,
+                             kk > 0 ? 1u : 0u);
+            umma_commit(&s_full[st]);
+            umma_commit(&k_empty[st]);
+        };
+        wait(q_full, 0);
+        scores(0);
+        for (int j = 0; j < n; j++) {
+            const int st = j & 1;
+            if (j + 1 < n) scores(j + 1);
+            wait(&v_full[st], j >> 1 & 1);
+            wait(&p_full[st], j >> 1 & 1);
+            tc_fence_after();
+            if (!dead)
+#pragma unroll
+                for (int kk = 0; kk < KEYS / 16; kk++)
+                    umma_f16_ts(t_o, t_s + st * KEYS + 8 * kk,
+                                sdesc_make(va + st * L::KBYTES + kk * 2048, KEYS * 128, 1024, LAYOUT_SW128), id_o,
+                                j > 0 || kk > 0 ? 1u : 0u);
+            umma_commit(&v_empty[st]);
+            umma_commit(o_done);
+        }
+        wait(o_done, (n - 1) & 1);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tmem, L::TMEM);
+}
+
+}  // namespace st
