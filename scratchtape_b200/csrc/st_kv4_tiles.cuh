@@ -144,20 +144,28 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
             const int st = j & 1, key0 = (first + j) * KEYS;
             wait(&s_full[st], j >> 1 & 1);
             tc_fence_after();
-            uint32_t x[KEYS];
-            tmem_ld32(t_s + lane_base + st * KEYS, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-            tmem_ld32(t_s + lane_base + st * KEYS + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
-            tmem_ld_wait();
             const uint32_t there = oks[j & 3];
-            if (key0 < all.x || key0 + KEYS > all.y || there != 15u) {
-                asm volatile("");
+            const bool edge = key0 < all.x || key0 + KEYS > all.y || there != 15u;
+            // half of the row's scores, hidden ones -inf
+            const auto half = [&](int c, uint32_t (&x)[32]) {
+                tmem_ld32(t_s + lane_base + st * KEYS + c, x);
+                tmem_ld_wait();
+                if (edge) {
+                    asm volatile("");
 #pragma unroll
-                for (int i = 0; i < KEYS; i++)
-                    if (key0 + i < sees.x || key0 + i >= sees.y || !(there >> (i / 16) & 1u)) x[i] = 0xff800000u;
-            }
+                    for (int i = 0; i < 32; i++)
+                        if (key0 + c + i < sees.x || key0 + c + i >= sees.y || !(there >> ((c + i) / 16) & 1u))
+                            x[i] = 0xff800000u;
+                }
+            };
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < KEYS; i++) top = fmaxf(top, __uint_as_float(x[i]));
+            for (int c = 0; c < KEYS; c += 32) {
+                uint32_t x[32];
+                half(c, x);
+#pragma unroll
+                for (int i = 0; i < 32; i++) top = fmaxf(top, __uint_as_float(x[i]));
+            }
             top *= c1;  // c1 > 0
             const bool move = top > -INFINITY && (!seen || top > ref + 8.0f);
             if (__any_sync(0xffffffffu, move)) {
@@ -181,15 +189,21 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                     }
                 }
             }
-            uint32_t p[32];
+            // read again rather than held: the weights of columns c, c + 1 go to
+            // column c / 2, over scores that have been read
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const float u = exp2_fast(fmaf(__uint_as_float(x[2 * i]), c1, -ref)),
-                            v = exp2_fast(fmaf(__uint_as_float(x[2 * i + 1]), c1, -ref));
-                l += u + v;
-                p[i] = pack2(u, v);
+            for (int c = 0; c < KEYS; c += 32) {
+                uint32_t x[32], p[16];
+                half(c, x);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float u = exp2_fast(fmaf(__uint_as_float(x[2 * i]), c1, -ref)),
+                                v = exp2_fast(fmaf(__uint_as_float(x[2 * i + 1]), c1, -ref));
+                    l += u + v;
+                    p[i] = pack2(u, v);
+                }
+                tmem_st16(t_s + lane_base + st * KEYS + c / 2, p);
             }
-            tmem_st32(t_s + lane_base + st * KEYS, p);
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&p_full[st]);
@@ -237,33 +251,42 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
         // values: the octet of channels and the words (four tokens each) of a tile's rows
         constexpr int OCT = D / 8, WORDS = D == 128 ? 2 : 1;
         const int oct = t % OCT, part = t / OCT, v_tile = part / (4 / WORDS), j0 = part % (4 / WORDS) * WORDS;
-        const auto page_of = [&](int tile) { return tile < n_tiles ? table[a.page_magic ? __umulhi(tile, a.page_magic) : tile] : -1; };
-        const auto at = [&](int tile, int page) -> const uint8_t * {
-            if (tile >= n_tiles || page < 0 || page >= a.n_pages) return nullptr;
-            const int in = tile - (a.page_magic ? __umulhi(tile, a.page_magic) : tile) * page_tiles;
-            return a.data + ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + in) * TILE;
-        };
-        uint32_t kw[KWORDS], vw[4][WORDS];
-        __half2 km[KG], vm[WORDS][4];
+        // lane l finds the place of the block's tile l % 4
+        const int lane = t & 31;
+        const auto quot = [&](int tile) { return a.page_magic ? __umulhi(tile, a.page_magic) : tile; };
+        uint32_t kw[KWORDS], vw[4][WORDS], vm[2][2 * WORDS];  // vm: tokens 2 j0 ..., and eight on
+        __half2 km[KG];
         uint32_t there = 0;
-        int k_page = -1, v_page = -1, lane_page = -1;
-        const auto pages = [&](int j) {  // of block j
-            const int tile = (first + j) * 4;
-            k_page = page_of(tile + key / 16);
-            v_page = page_of(tile + v_tile);
-            lane_page = page_of(tile + (t & 3));
+        int page = -1;
+        const auto find = [&](int j) {  // the page of block j's tile
+            const int tile = (first + j) * 4 + (lane & 3);
+            page = tile < n_tiles ? table[quot(tile)] : -1;
         };
         const auto load = [&](int j) {  // block j's codes to registers
-            const int tile = (first + j) * 4, k_tile = tile + key / 16;
-            const uint8_t *p = at(k_tile, k_page), *q = at(tile + v_tile, v_page);
+            const int tile0 = (first + j) * 4, tile = tile0 + (lane & 3);
+            const bool ok = page >= 0 && page < a.n_pages;
+            if (t < 4 && tile < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
+            const uint32_t have = __ballot_sync(0xffffffffu, ok) & 15u;
+            there = have | (__ballot_sync(0xffffffffu, tile >= n_tiles) & 15u);
+            const int64_t off = ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + (tile - quot(tile) * page_tiles)) * TILE;
+            const uint8_t *p = a.data + __shfl_sync(0xffffffffu, off, key >> 4), *q = a.data + __shfl_sync(0xffffffffu, off, v_tile);
             const int r = key & 15;
-            const bool here = p && k_tile * 16 + r < s.len;
+            const bool here = have >> (key >> 4) & 1u, v_here = have >> v_tile & 1u;
+            constexpr int PER = KWORDS / KG;
+            if (have != 15u) {
+                asm volatile("");
 #pragma unroll
-            for (int i = 0; i < KWORDS; i++) kw[i] = 0;
+                for (int i = 0; i < KWORDS; i++) kw[i] = 0;
 #pragma unroll
-            for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
+                for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < WORDS; w++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) vw[i][w] = 0;
+                    vm[0][2 * w] = vm[0][2 * w + 1] = vm[1][2 * w] = vm[1][2 * w + 1] = 0;
+                }
+            }
             if (here) {
-                constexpr int PER = KWORDS / KG;
 #pragma unroll
                 for (int g = 0; g < KG; g++) {
                     const int c = c0 + g * (HALF / KG);
@@ -276,28 +299,30 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                     km[g] = reinterpret_cast<const __half2 *>(p + kv4_kmeta(D))[(c / G) * 16 + r];
                 }
             }
+            if (v_here) {
+                const uint8_t *codes = q + kv4_val(D) + oct * 64 + 4 * j0;
+                const uint8_t *meta = q + kv4_vmeta(D, G) + ((oct * 8 / G) * 16 + 2 * j0) * 4;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++) memcpy(vw[i], __builtin_assume_aligned(codes + 16 * i, 4 * WORDS), 4 * WORDS);
 #pragma unroll
-                for (int w = 0; w < WORDS; w++)
-                    vw[i][w] = q ? *reinterpret_cast<const uint32_t *>(q + kv4_val(D) + (oct * 4 + i) * 16 + 4 * (j0 + w)) : 0;
+                for (int i = 0; i < 2; i++) memcpy(vm[i], __builtin_assume_aligned(meta + 32 * i, 8 * WORDS), 8 * WORDS);
+            }
+            if ((tile0 + 4) * 16 > s.len) {  // tokens past the end: whatever their slots hold counts for 0
+                asm volatile("");
+                if (tile0 * 16 + key >= s.len)
 #pragma unroll
-            for (int w = 0; w < WORDS; w++)
+                    for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int token = 2 * (j0 + w) + (k & 1) * 8 + (k >> 1);
-                    const bool real = q && (tile + v_tile) * 16 + token < s.len;
-                    vm[w][k] = real ? reinterpret_cast<const __half2 *>(q + kv4_vmeta(D, G))[(oct * 8 / G) * 16 + token]
-                                    : __floats2half2_rn(0.0f, 0.0f);
-                }
-            const bool ok = lane_page >= 0 && lane_page < a.n_pages;
-            if (t < 4 && tile + t < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
-            there = __ballot_sync(0xffffffffu, ok || tile + (t & 3) >= n_tiles) & 15u;
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int k = 0; k < 2 * WORDS; k++)
+                        if ((tile0 + v_tile) * 16 + 2 * j0 + 8 * i + k >= s.len) vm[i][k] = 0;
+            }
         };
         if (n > 0) {
-            pages(0);
+            find(0);
             load(0);
-            if (n > 1) pages(1);
+            if (n > 1) find(1);
         }
         for (int j = 0; j < n; j++) {
             const int st = j & 1;
@@ -324,15 +349,16 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int row = v_tile * 16 + 2 * (j0 + w) + (k & 1) * 8 + (k >> 1);
+                    const __half2 m = *reinterpret_cast<const __half2 *>(&vm[k & 1][2 * w + (k >> 1)]);
                     *reinterpret_cast<uint4 *>(vs + oct / 8 * (KEYS * 128) + sw128_offset(row, oct % 8)) =
-                        kv4_expand(tok[k], __low2half2(vm[w][k]), __high2half2(vm[w][k]));
+                        kv4_expand(tok[k], __low2half2(m), __high2half2(m));
                 }
             }
             fence_proxy_async_smem();
             mbar_arrive(&v_full[st]);
             if (j + 1 < n) {
                 load(j + 1);
-                if (j + 2 < n) pages(j + 2);
+                if (j + 2 < n) find(j + 2);
             }
         }
     } else if (tid == 256 && n > 0) {
