@@ -15,6 +15,7 @@
 // 8-column one, so shared heads fill the columns and each cached byte is read
 // once, by one thread.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "st_kv4_attn.cuh"
@@ -745,7 +746,6 @@ template <typename T, int D, int G, int NT>
 st_status launch(st_handle *h, AttnArgs a) {
     using S = Shape<T, D, G, NT>;
     const Plan plan(h, a.batch, a.rows, a.max_q, a.kv_heads, a.share, NT, a.max_pages * a.page, S::TEAMS);
-    a.sms = h->num_sms;
     a.parts = static_cast<int>(plan.parts);
     a.item_blocks = plan.item_blocks;
     a.notes = plan.notes;
@@ -762,10 +762,23 @@ st_status launch(st_handle *h, AttnArgs a) {
     return st_after_launch(h, "k_kv4_attn_join");
 }
 
-// Many rows of 16-bit types go by tiles of 128 (a positive scale: the largest
-// score is the largest product).
-bool by_tiles(const AttnArgs &a, int dtype) {
-    return dtype != ST_F32 && a.scale_log2 > 0.0f && a.max_q * static_cast<int64_t>(a.share) >= 32 && a.batch <= 65535;
+// Whether rows of 16-bit types go by tiles of 128 (with a positive scale: the
+// largest score is the largest product).  A tile goes through its keys alone,
+// so it takes many tiles, or few keys, to be ahead of the kernel that cuts
+// the keys for all teams.  Both as measured, in us: a block of 64 keys takes a tile
+// 1.15 where it has its SM alone and 1.75 where two share one; the teams
+// together do 785 steps of 32 keys and 16 rows a us (1300 at d = 64) after a start of
+// 14.  E.g. 32 heads on 8, d 128: one sequence of 8192 keys, 128 rows 149 by tiles
+// and 96 by teams, 256 rows 148 and 175, 1024 rows 211 and 668; 16 sequences of
+// 4096, 8 rows each 80 and 56, 16 rows 80 and 99.
+bool by_tiles(const AttnArgs &a) {
+    const int64_t rows = a.max_q * static_cast<int64_t>(a.share), keys = a.max_pages * a.page;
+    if (a.scale_log2 <= 0.0f || rows <= 16 || a.batch > 65535) return false;
+    const double seqs = static_cast<double>(a.batch) * a.kv_heads;
+    const double tiles = seqs * static_cast<double>((rows + 127) / 128);
+    const double by_tile = 5.0 + keys / 64.0 * (tiles <= a.sms ? 1.15 : 1.75 * std::ceil(tiles / (2.0 * a.sms)));
+    const double steps = seqs * static_cast<double>((rows + 15) / 16) * (keys / 32.0);
+    return by_tile < 14.0 + steps / (a.d == 128 ? 785.0 : 1300.0);
 }
 
 template <typename T, int D, int G>
@@ -782,7 +795,7 @@ st_status launch_tiles(st_handle *h, const AttnArgs &a) {
 template <typename T, int D, int G>
 st_status by_columns(st_handle *h, const AttnArgs &a, int nt) {
     if constexpr (sizeof(T) == 2)
-        if (by_tiles(a, std::is_same<T, __half>::value ? ST_F16 : ST_BF16)) return launch_tiles<T, D, G>(h, a);
+        if (by_tiles(a)) return launch_tiles<T, D, G>(h, a);
     return nt == 1 ? launch<T, D, G, 1>(h, a) : launch<T, D, G, 2>(h, a);
 }
 
@@ -832,9 +845,9 @@ extern "C" st_status st_kv4_attn(st_handle *h, const void *q, int64_t q_token, i
     const int size = dtype == ST_F32 ? 4 : 2;
     const int vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token * size % 16 == 0 && q_head * size % 16 == 0;
     const AttnArgs a = {q, q_token, q_head, o, lse, static_cast<const uint8_t *>(data), n_pages, page, heads,
-                        kv_heads, share, pages, max_pages, kv_len, q_start, batch, rows, static_cast<int>(max_q),
+                        kv_heads, share, d, pages, max_pages, kv_len, q_start, batch, rows, static_cast<int>(max_q),
                         page == 16 ? 0u : static_cast<uint32_t>(((1ull << 32) + page / 16 - 1) / (page / 16)),
-                        scale * 1.44269504088896341f, causal, one, window, vec, 0, 0, 0, 0, static_cast<float *>(workspace),
+                        scale * 1.44269504088896341f, causal, one, window, vec, h->num_sms, 0, 0, 0, static_cast<float *>(workspace),
                         h->d_status};
 #define KV4_CASE(D_, G_)                                                               \
     if (d == D_ && group == G_) {                                                      \
