@@ -8,12 +8,19 @@
 // With codes c, scales s and zeros z by groups g of channels,
 //     q . k_j = sum_g s_jg (q_g . c_jg) + z_jg sum(q_g)
 //     o_g     = sum_j (p_j s_jg) c_jg + sum_j p_j z_jg
-// so the tensor cores multiply the codes themselves: a code in the low bits of
-// an f16 is the subnormal c 2^-24 (four bits further up, c 2^-20), exact, and
-// one AND makes two operands of mma.sync.  Codes are the 16-row operand (keys:
-// tokens x channels, values: channels x tokens), queries and weights the
-// 8-column one, so shared heads fill the columns and each cached byte is read
-// once, by one thread.
+// so the tensor cores multiply the codes themselves, in one of two forms.  A code
+// in the low bits of an f16 is the subnormal c 2^-24 (four bits further up, c
+// 2^-20), and one AND makes two of them; but products lose what lies ten bits
+// below an operand's first possible bit, and sums come out off by 3e-5 of
+// themselves, 8e-4 of a result over 131,000 keys: half of what rounding it to bf16
+// does, four times what rounding it to f16 does.  So that form serves bf16 results
+// without a log-sum-exp.  EXACT, for all others: 1024 + c is made by an AND and
+// OR, and a subtraction leaves c - 8 exactly (z + 8 s makes up for it, and the
+// sums, which are truncated as they grow, stay small): 3e-7 in f32.  The
+// subtractions take a third of the time again (64 x 16k keys: 206 us and 280).
+// Codes are the 16-row operand of mma.sync (keys: tokens x channels, values:
+// channels x tokens), queries and weights the 8-column one, so shared heads fill
+// the columns and each cached byte is read once, by one thread.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -129,6 +136,25 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The codes of nibbles 0 and 4 of w, and of 1 and 5: EXACT less 8, else times
+// 2^-24 and 2^-20.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t codes04(uint32_t w) {
+    if (!EXACT) return w & 0x000f000fu;
+    w = (w & 0x000f000fu) | 0x64006400u;  // 1024 + c
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&w),
+                              __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));  // 1032
+    return *reinterpret_cast<const uint32_t *>(&x);
+}
+template <bool EXACT>
+__device__ __forceinline__ uint32_t codes15(uint32_t w) {
+    if (!EXACT) return w & 0x00f000f0u;
+    w = (w & 0x00f000f0u) | 0x64006400u;  // 1024 + 16 c
+    const __half2 x = __hfma2(*reinterpret_cast<const __half2 *>(&w),
+                              __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00)),    // 1 / 16
+                              __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480)));  // -72
+    return *reinterpret_cast<const uint32_t *>(&x);
+}
 // The same from zero.
 __device__ __forceinline__ void mma_f16_0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
@@ -191,7 +217,7 @@ __device__ __forceinline__ void finish(const AttnArgs &a, int64_t first, int hea
 // warps' results are joined at the end of a piece.  An item that one team
 // holds whole is written out; parts of one go to the workspace and are joined
 // by k_kv4_attn_join, which finds them by the notes that the parts leave.
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, bool EXACT>
 __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_kv4_attn(const AttnArgs a) {
     using S = Shape<T, D, G, NT>;
     constexpr int NG = S::NG, RB = S::RB, TILE = S::TILE, STAGES = S::STAGES, KS = G / 16, MT = D / 16;
@@ -322,8 +348,7 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
         team_sync();
         const int top_exp = static_cast<int>(max(max(q_tops[team][0], q_tops[team][1]), max(q_tops[team][2], q_tops[team][3])) >> 23);
         const int up = top_exp > 0 ? max(-100, min(100, 14 + 127 - top_exp)) : 0;
-        // a code is c 2^-24 (c 2^-20 in the upper nibbles: those channels take q / 16)
-        const float c1 = __uint_as_float(static_cast<uint32_t>(24 - up + 127) << 23) * a.scale_log2;
+        const float c1 = __uint_as_float(static_cast<uint32_t>((EXACT ? 0 : 24) + 127 - up) << 23) * a.scale_log2;
         const float up_mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
@@ -332,7 +357,7 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
             uint32_t high[4], low[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {  // channels k and k + 4
-                const float f = k & 1 ? up_mul * 0.0625f : up_mul;
+                const float f = !EXACT && (k & 1) ? up_mul * 0.0625f : up_mul;  // against codes times 2^-20
                 const float u = xq[i][k] * f, v = xq[i][k + 4] * f;
                 high[k] = pack2(u, v);
                 const float2 r2 = unpack2(high[k]);
@@ -424,8 +449,7 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
                             const uint32_t va = wa[w] >> (8 * k), vb = wb[w] >> (8 * k);
-                            const uint32_t a0 = va & 0x000f000fu, a1 = vb & 0x000f000fu, a2 = va & 0x00f000f0u,
-                                           a3 = vb & 0x00f000f0u;
+                            const uint32_t a0 = codes04<EXACT>(va), a1 = codes04<EXACT>(vb), a2 = codes15<EXACT>(va), a3 = codes15<EXACT>(vb);
 #pragma unroll
                             for (int qs = QS - 1; qs >= 0; qs--)
 #pragma unroll
@@ -439,6 +463,7 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
                         }
                     const uint32_t *meta = reinterpret_cast<const uint32_t *>(tp + kv4_kmeta(D)) + gr * 16 + g;
                     float2 ma = unpack2(meta[0]), mb = unpack2(meta[8]);
+                    if (EXACT) ma.y = fmaf(8.0f, ma.x, ma.y), mb.y = fmaf(8.0f, mb.x, mb.y);
                     ma.x *= c1, mb.x *= c1;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
@@ -550,7 +575,8 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
                     for (int gr = 0; gr < NG; gr++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const float2 sz = unpack2(vm[tile][gr][h]);
+                            float2 sz = unpack2(vm[tile][gr][h]);
+                            if (EXACT) sz.y = fmaf(8.0f, sz.x, sz.y);
                             const float u = p[2 * h] * sz.x, v = p[2 * h + 1] * sz.x;
                             const uint32_t w = pack2(u, v);
                             pf[0][nt][gr][h] = transpose8(w);
@@ -566,8 +592,7 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
 #pragma unroll
                 for (int i2 = 0; i2 < MT; i2++) {
                     const uint32_t va = vp[i2 * 32], vb = va >> 8;
-                    const uint32_t a0 = va & 0x000f000fu, a1 = va & 0x00f000f0u, a2 = vb & 0x000f000fu,
-                                   a3 = vb & 0x00f000f0u;
+                    const uint32_t a0 = codes04<EXACT>(va), a1 = codes15<EXACT>(va), a2 = codes04<EXACT>(vb), a3 = codes15<EXACT>(vb);
                     constexpr int PER = MT / NG;
 #pragma unroll
                     for (int qs = QS - 1; qs >= 0; qs--)
@@ -600,7 +625,8 @@ __global__ void __launch_bounds__(Shape<T, D, G, NT>::TEAMS * WARPS * 32, 1) k_k
 #pragma unroll
                     for (int i2 = gr * PER; i2 < (gr + 1) * PER; i2++)
                         *reinterpret_cast<float2 *>(mine + row * D + 16 * i2 + 2 * g) =
-                            make_float2(fmaf(acc[nt][i2][e], 0x1p24f, zs), fmaf(acc[nt][i2][e + 2], 0x1p20f, zs));
+                            make_float2(fmaf(acc[nt][i2][e], EXACT ? 1.0f : 0x1p24f, zs),
+                                        fmaf(acc[nt][i2][e + 2], EXACT ? 1.0f : 0x1p20f, zs));
                 }
                 if (g == 0) {
                     mine[RB * D + row] = ls > 0.0f || ls != ls ? -neg[nt][e] : -INFINITY;
@@ -742,16 +768,16 @@ struct Plan {
     }
 };
 
-template <typename T, int D, int G, int NT>
+template <typename T, int D, int G, int NT, bool EXACT>
 st_status launch(st_handle *h, AttnArgs a) {
     using S = Shape<T, D, G, NT>;
     const Plan plan(h, a.batch, a.rows, a.max_q, a.kv_heads, a.share, NT, a.max_pages * a.page, S::TEAMS);
     a.parts = static_cast<int>(plan.parts);
     a.item_blocks = plan.item_blocks;
     a.notes = plan.notes;
-    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_kv4_attn<T, D, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    ST_CHECK_CUDA(h, cudaFuncSetAttribute(k_kv4_attn<T, D, G, NT, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           S::TEAMS * S::SMEM));
-    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn<T, D, G, NT>, dim3(static_cast<unsigned>(std::min<int64_t>(plan.parts, h->num_sms))),
+    ST_CHECK_CUDA(h, st_launch_dependent(h, k_kv4_attn<T, D, G, NT, EXACT>, dim3(static_cast<unsigned>(std::min<int64_t>(plan.parts, h->num_sms))),
                                          dim3(S::TEAMS * WARPS * 32), S::TEAMS * S::SMEM, a));
     if (st_status s = st_after_launch(h, "k_kv4_attn"); s != ST_OK || plan.parts == 1) return s;
     const dim3 notes(static_cast<unsigned>(plan.notes), plan.deep ? S::RB / 2 : 1);
@@ -762,8 +788,9 @@ st_status launch(st_handle *h, AttnArgs a) {
     return st_after_launch(h, "k_kv4_attn_join");
 }
 
-// Whether rows of 16-bit types go by tiles of 128 (with a positive scale: the
-// largest score is the largest product).  A tile goes through its keys alone,
+// Whether bf16 rows go by tiles of 128 (with a positive scale: the largest score
+// is the largest product; without a log-sum-exp, for which scores of rounded
+// keys are 1e-5 of it off).  A tile goes through its keys alone,
 // so it takes many tiles, or few keys, to be ahead of the kernel that cuts
 // the keys for all teams.  Both as measured, in us: a block of 64 keys takes a tile
 // 1.15 where it has its SM alone and 1.75 where two share one; the teams
@@ -773,13 +800,18 @@ st_status launch(st_handle *h, AttnArgs a) {
 // 4096, 8 rows each 80 and 56, 16 rows 80 and 99.
 bool by_tiles(const AttnArgs &a) {
     const int64_t rows = a.max_q * static_cast<int64_t>(a.share), keys = a.max_pages * a.page;
-    if (a.scale_log2 <= 0.0f || rows <= 16 || a.batch > 65535) return false;
+    if (a.scale_log2 <= 0.0f || a.lse || rows <= 16 || a.batch > 65535) return false;
     const double seqs = static_cast<double>(a.batch) * a.kv_heads;
     const double tiles = seqs * static_cast<double>((rows + 127) / 128);
     const double by_tile = 5.0 + keys / 64.0 * (tiles <= a.sms ? 1.15 : 1.75 * std::ceil(tiles / (2.0 * a.sms)));
     const double steps = seqs * static_cast<double>((rows + 15) / 16) * (keys / 32.0);
     return by_tile < 14.0 + steps / (a.d == 128 ? 785.0 : 1300.0);
 }
+
+// Tiles round keys to f16, which bf16 results do not show (1.75e-3 off against
+// 1.66e-3 for the rounding alone) and f16 ones would (6e-4 against 2e-4).
+template <typename T>
+constexpr bool TILED = std::is_same<T, __nv_bfloat16>::value;
 
 template <typename T, int D, int G>
 st_status launch_tiles(st_handle *h, const AttnArgs &a) {
@@ -794,9 +826,11 @@ st_status launch_tiles(st_handle *h, const AttnArgs &a) {
 
 template <typename T, int D, int G>
 st_status by_columns(st_handle *h, const AttnArgs &a, int nt) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (TILED<T>)
         if (by_tiles(a)) return launch_tiles<T, D, G>(h, a);
-    return nt == 1 ? launch<T, D, G, 1>(h, a) : launch<T, D, G, 2>(h, a);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        if (!a.lse) return nt == 1 ? launch<T, D, G, 1, false>(h, a) : launch<T, D, G, 2, false>(h, a);
+    return nt == 1 ? launch<T, D, G, 1, true>(h, a) : launch<T, D, G, 2, true>(h, a);
 }
 
 }  // namespace

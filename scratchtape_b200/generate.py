@@ -1,0 +1,116 @@
+"""Token generation with a trained ``TinyLM``: the decoding step over a 4-bit paged cache.
+
+Each step takes one token of every sequence through the model's blocks (lm.py: the same weights, LayerNorm,
+projections and head), appends its keys and values to a cache per layer (``kv4.append``; the model has learned
+positions, so nothing is rotated), attends over the cache (``kv4.attend``), adjusts the logits by each sequence's
+penalties, biases and mask (``logits.adjust``) and takes the largest.  A prompt goes through the same path,
+all its tokens at once.  Sequences may have different lengths; pages are given out as they grow.
+"""
+import torch
+
+from . import kv4, logits
+from .device import handle, ptr
+from .lm import TinyLM
+from .matmul import Epilogue, MatRef, matmul_with
+
+
+class Generator:
+    """Decodes ``batch`` sequences of up to ``model.c.t`` tokens; pages of ``page`` tokens, groups of ``group``
+    channels.  Penalties as in ``logits.adjust``, one value for all sequences (None: none)."""
+
+    def __init__(self, model: TinyLM, batch: int, page: int = 16, group: int = 64, repetition=None, presence=None,
+                 frequency=None, bias=None, mask=None):
+        c = model.c
+        self.m, self.batch, self.page, self.group, self.d = model, batch, page, group, c.d // c.heads
+        dev = model.device
+        most = -(-c.t // page)
+        self.cache = [kv4.empty(batch * most, page, c.heads, self.d, group, dev) for _ in range(c.layers)]
+        # a sequence's pages are the batch's in turn: consecutive tokens are not neighbours in memory
+        self.pages = torch.arange(batch * most, dtype=torch.int32, device=dev).view(most, batch).t().contiguous()
+        self.length = torch.zeros(batch, dtype=torch.int64)  # tokens in the cache, on the host
+        self.kv_len = torch.zeros(batch, dtype=torch.int32, device=dev)
+        row = lambda x: None if x is None else torch.full((batch,), float(x), device=dev)  # noqa: E731
+        self.penalties = row(repetition), row(presence), row(frequency)
+        self.bias, self.mask = bias, mask
+        self.history = [[] for _ in range(batch)]
+        self.prompt = [0] * batch
+
+    def _linear(self, x, w, b, rows, k, n, relu=False, residual=None):
+        out = torch.empty((rows, n), dtype=torch.float32, device=x.device)
+        matmul_with(MatRef(x), MatRef(w), MatRef(out), 1, rows, k, n,
+                    Epilogue(bias=(b, 0), relu=relu, residual=None if residual is None else (residual, 0)),
+                    self.m.c.gemm_prec)
+        return out
+
+    def _norm(self, x, name):
+        p, y = self.m.p, torch.empty_like(x)
+        mean, rstd = (torch.empty(x.shape[0], dtype=torch.float32, device=x.device) for _ in range(2))
+        handle(x.device).call("st_layernorm_fwd", ptr(x), ptr(p[name + "_g"]), ptr(p[name + "_b"]), ptr(y), ptr(mean),
+                              ptr(rstd), x.shape[0], x.shape[1], self.m.c.ln_eps)
+        return y
+
+    def forward(self, tokens):
+        """tokens: a list of new tokens for each sequence (possibly none).  Appends them and returns the logits
+        [batch, vocab] after each sequence's last one, as they are (a row of a sequence without new tokens means
+        nothing)."""
+        c, p, dev = self.m.c, self.m.p, self.m.device
+        counts = [len(t) for t in tokens]
+        new = torch.tensor(counts, dtype=torch.int64)
+        if int((self.length + new).max()) > c.t:
+            raise ValueError("sequences of more than %d tokens" % c.t)
+        rows = int(new.sum())
+        if rows == 0:
+            raise ValueError("no tokens")
+        seq = torch.repeat_interleave(torch.arange(self.batch), new)
+        start = torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)])
+        pos = self.length[seq] + torch.arange(rows) - start[seq]
+        seq, pos, start = seq.to(dev), pos.to(dev), start.to(dev)
+        slots = self.pages[seq, pos // self.page].long() * self.page + pos % self.page
+        ids = torch.tensor([v for t in tokens for v in t], dtype=torch.int64, device=dev)
+        self.length += new
+        self.kv_len.copy_(self.length)
+        x = p["tok"][ids] + p["pos"][pos]
+        q_start, max_q = start.to(torch.int32), max(counts)
+        for i in range(c.layers):
+            w = "l%d." % i
+            qkv = self._linear(self._norm(x, w + "ln1"), p[w + "wqkv"], p[w + "bqkv"], rows, c.d, 3 * c.d)
+            q, k, v = qkv.view(rows, 3, c.heads, self.d).unbind(1)  # views: rows of the fused projection
+            kv4.append(self.cache[i], k, v, slots, self.group)
+            o = kv4.attend(q, self.cache[i], self.pages, self.kv_len, self.d ** -0.5, self.group, q_start=q_start,
+                           max_q=max_q, one=c.softmax1)
+            x = self._linear(o.view(rows, c.d), p[w + "wo"], p[w + "bo"], rows, c.d, c.d, residual=x)
+            hid = self._linear(self._norm(x, w + "ln2"), p[w + "w1"], p[w + "b1"], rows, c.d, c.dff, relu=True)
+            x = self._linear(hid, p[w + "w2"], p[w + "b2"], rows, c.dff, c.d, residual=x)
+        last = self._norm(x[(start[1:] - 1).clamp(min=0)].contiguous(), "lnf")
+        out = torch.empty((self.batch, c.vocab), dtype=torch.float32, device=dev)
+        matmul_with(MatRef(last), MatRef(p["tok"], trans=True), MatRef(out), 1, self.batch, c.d, c.vocab, None, c.gemm_prec)
+        return out
+
+    def step(self, tokens):
+        """Appends each sequence's new tokens; returns (its next token int64 [batch], the adjusted logits).
+        Tokens of the first call are the prompt."""
+        dev = self.m.device
+        for b, t in enumerate(tokens):
+            if not self.history[b]:
+                self.prompt[b] = len(t)
+            self.history[b] += [int(v) for v in t]
+        raw = self.forward(tokens)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+        starts = [0]
+        for h in self.history:
+            starts.append(starts[-1] + len(h))
+        repetition, presence, frequency = self.penalties
+        out = logits.adjust(raw, i32([v for h in self.history for v in h]), i32(starts), i32(self.prompt), repetition,
+                            presence, frequency, bias=self.bias, mask=self.mask, out=raw)
+        return out.argmax(1), out
+
+    def generate(self, prompts, steps: int):
+        """Greedy continuations of the prompts (lists of tokens): a list of ``steps`` tokens for each."""
+        got = [[] for _ in prompts]
+        tokens = prompts
+        for _ in range(steps):
+            best, _ = self.step(tokens)
+            tokens = [[int(v)] for v in best.tolist()]
+            for g, t in zip(got, tokens):
+                g += t
+        return got

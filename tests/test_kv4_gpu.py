@@ -181,7 +181,77 @@ def test_attend(dev, case):
     again, lse2 = kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **args)
     assert torch.equal(o, again) and torch.equal(lse, lse2)
     assert dev.last_kernel.startswith("k_kv4_")
+    alone = kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **dict(args, return_lse=False))
+    close(alone, want, vmax, dtype)  # bf16 goes another way without a log-sum-exp
     dev.sync()
+
+
+TILED = [
+    # lens, rows of each, heads, kv_heads, d, group, page, causal, window, one: many rows of bf16
+    ([900], [900], 8, 2, 128, 64, 64, True, 0, False),
+    ([513, 700], [513, 128], 16, 4, 128, 128, 16, True, 0, True),
+    ([640, 1000, 65, 0, 300], [300, 257, 65, 40, 310], 8, 1, 128, 32, 48, True, 70, False),
+    ([700, 20, 511], [500, 450, 1], 12, 2, 64, 64, 32, True, 0, False),
+    ([333, 900], [333, 640], 7, 1, 64, 32, 128, False, 0, True),
+    ([1200], [600], 5, 5, 128, 64, 16, False, 200, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(TILED)))
+@pytest.mark.parametrize("aligned", [True, False])
+def test_attend_by_tiles(dev, case, aligned):
+    """Many rows of bf16, queries in rows of a wider tensor, on 16-byte boundaries or not."""
+    lens, counts, heads, kv_heads, d, group, page, causal, window, one = TILED[case]
+    data, pages = filled(lens, kv_heads, d, group, page, 50 + case)
+    g = torch.Generator(device=DEV).manual_seed(case)
+    off = 8 if aligned else 3
+    wide = torch.randn((sum(counts), heads * d + 2 * off), generator=g, device=DEV).to(BF16) * 2
+    q = wide[:, off:off + heads * d].unflatten(1, (heads, d))
+    start = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    args = dict(q_start=start, max_q=max(counts), causal=causal, one=one, window=window)
+    o = kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **args)
+    assert dev.last_kernel == "k_kv4_attn_tiles"
+    want, _, vmax = attend64(q, data, pages, lens, counts, d ** -0.5, group, causal, window, one)
+    close(o, want, vmax, BF16)
+    assert torch.equal(o, kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **args))
+    dev.sync()
+
+
+def test_tiles_and_a_page_outside_the_cache(dev):
+    """Keys of a page number out of range are left out and reported, by either kernel; a score far above those
+    before it, and rows whose first keys are hidden, rescale what was summed."""
+    import scratchtape_b200._native as N
+    d, group, page, n = 128, 64, 32, 640
+    data, pages = filled([n], 2, d, group, page, 9)
+    k = torch.randn((n, 2, d), device=DEV, generator=torch.Generator(device=DEV).manual_seed(4))
+    k[300] *= 30.0
+    k[500] *= 90.0
+    v = torch.randn((n, 2, d), device=DEV, generator=torch.Generator(device=DEV).manual_seed(5))
+    kv4().append(data, k, v, slots_of(pages, 0, 0, n, page), group)
+    q = torch.randn((n, 8, d), device=DEV, generator=torch.Generator(device=DEV).manual_seed(6)).to(BF16)
+    start = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor([n], dtype=torch.int32, device=DEV)
+    call = lambda p, **a: kv4().attend(q, data, p, kv_len, 0.1, group, q_start=start, **a)  # noqa: E731
+    o = call(pages)
+    assert dev.last_kernel == "k_kv4_attn_tiles"
+    want, _, vmax = attend64(q, data, pages, [n], [n], 0.1, group, True, 0, False)
+    close(o, want, vmax, BF16)
+    dev.sync()
+    wrong = pages.clone()
+    wrong[0, 3], wrong[0, 7] = data.shape[0], -1
+    for a in ({}, {"return_lse": True}):
+        got = call(wrong, **a)
+        with pytest.raises(N.StError, match="INVALID_ARG"):
+            dev.sync()
+        dev.sync()
+        got = got[0] if a else got
+        assert torch.isfinite(got).all()
+        close(got[:96], want[:96], vmax, BF16)  # rows that do not see them
+        hidden = [j for j in range(n) if j // page not in (3, 7)]
+        kk, vv = (x[slots_of(pages, 0, 0, n, page)][hidden].repeat_interleave(4, 1) for x in values64(data, d, group))
+        x = torch.einsum("hd,jhd->hj", q[n - 1].double(), kk) * 0.1
+        close(got[n - 1], torch.einsum("hj,jhd->hd", torch.softmax(x, -1), vv), vmax, BF16)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
