@@ -788,9 +788,8 @@ st_status launch(st_handle *h, AttnArgs a) {
     return st_after_launch(h, "k_kv4_attn_join");
 }
 
-// Whether bf16 rows go by tiles of 128 (with a positive scale: the largest score
-// is the largest product; without a log-sum-exp, for which scores of rounded
-// keys are 1e-5 of it off).  A tile goes through its keys alone,
+// Whether rows of 16-bit types go by tiles of 128 (with a positive scale: the
+// largest score is the largest product).  A tile goes through its keys alone,
 // so it takes many tiles, or few keys, to be ahead of the kernel that cuts
 // the keys for all teams.  Both as measured, in us: a block of 64 keys takes a tile
 // 1.15 where it has its SM alone and 1.75 where two share one; the teams
@@ -800,18 +799,13 @@ st_status launch(st_handle *h, AttnArgs a) {
 // 4096, 8 rows each 80 and 56, 16 rows 80 and 99.
 bool by_tiles(const AttnArgs &a) {
     const int64_t rows = a.max_q * static_cast<int64_t>(a.share), keys = a.max_pages * a.page;
-    if (a.scale_log2 <= 0.0f || a.lse || rows <= 16 || a.batch > 65535) return false;
+    if (a.scale_log2 <= 0.0f || rows <= 16 || a.batch > 65535) return false;
     const double seqs = static_cast<double>(a.batch) * a.kv_heads;
     const double tiles = seqs * static_cast<double>((rows + 127) / 128);
     const double by_tile = 5.0 + keys / 64.0 * (tiles <= a.sms ? 1.15 : 1.75 * std::ceil(tiles / (2.0 * a.sms)));
     const double steps = seqs * static_cast<double>((rows + 15) / 16) * (keys / 32.0);
     return by_tile < 14.0 + steps / (a.d == 128 ? 785.0 : 1300.0);
 }
-
-// Tiles round keys to f16, which bf16 results do not show (1.75e-3 off against
-// 1.66e-3 for the rounding alone) and f16 ones would (6e-4 against 2e-4).
-template <typename T>
-constexpr bool TILED = std::is_same<T, __nv_bfloat16>::value;
 
 template <typename T, int D, int G>
 st_status launch_tiles(st_handle *h, const AttnArgs &a) {
@@ -826,7 +820,7 @@ st_status launch_tiles(st_handle *h, const AttnArgs &a) {
 
 template <typename T, int D, int G>
 st_status by_columns(st_handle *h, const AttnArgs &a, int nt) {
-    if constexpr (TILED<T>)
+    if constexpr (sizeof(T) == 2)
         if (by_tiles(a)) return launch_tiles<T, D, G>(h, a);
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (!a.lse) return nt == 1 ? launch<T, D, G, 1, false>(h, a) : launch<T, D, G, 2, false>(h, a);

@@ -8,12 +8,15 @@
 // products, and four warps, a thread a row, take the scores from TMEM to
 // weights and put them back into the same TMEM columns as the A operand of the
 // second product.  Two blocks share an SM, so one's products run while the
-// other's softmax does (the exponentials take about as long as the products:
-// 64 x 128 of them at 16 a clock against 2 x 128 x 64 x d multiplies).
+// other's softmax does (the exponentials take about as long as the products).
 //
-// Roundings: queries are exact in f16 (a power of two per row), c * scale +
-// zero is rounded to f16 once (2^-12 of a key or value), weights to f16.
+// Roundings: queries are exact in f16 (a power of two per row), keys in two terms
+// of f16 (with one, scores were off by 2^-12 of themselves, which f16 results,
+// log-sum-exps and large scores show), values c * scale + zero are rounded to f16, and so
+// are weights, but in two terms where the result is f16.
 #pragma once
+#include <type_traits>
+
 #include "st_kv4_attn.cuh"
 
 namespace st {
@@ -41,11 +44,33 @@ __device__ __forceinline__ uint4 kv4_expand(uint32_t w, __half2 s, __half2 z) {
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
+// The same in two terms of f16: low is what rounding high leaves, exactly.
+__device__ __forceinline__ void kv4_expand2(uint32_t w, __half2 s, __half2 z, uint4 &high, uint4 &low) {
+    const __half2 k1024 = __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x6400));
+    const __half2 sixteenth = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));
+    const __half2 down = __halves2half2(__ushort_as_half(0xd400), __ushort_as_half(0xd400));
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t v = w >> (8 * (k / 2)), a = (v & (k & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+        const __half2 x = *reinterpret_cast<const __half2 *>(&a);
+        const __half2 c = k & 1 ? __hfma2(x, sixteenth, down) : __hsub2(x, k1024);
+        const __half2 p = __hmul2_rn(c, s), e = __hfma2(c, s, __hneg2(p));  // c s = p + e
+        const __half2 sum = __hadd2_rn(p, z), zz = __hsub2_rn(sum, p);       // p + z = sum + the rest
+        const __half2 rest = __hadd2_rn(__hsub2_rn(p, __hsub2_rn(sum, zz)), __hsub2_rn(z, zz));
+        const __half2 r = __hadd2_rn(rest, e);
+        h[k] = *reinterpret_cast<const uint32_t *>(&sum);
+        l[k] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+    high = make_uint4(h[0], h[1], h[2], h[3]);
+    low = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
 template <typename T, int D, int G>
 struct Tiles {
     static constexpr int ROWS = 128, KEYS = 64, CHUNKS = D / 64;
     static constexpr int Q = 0, K = Q + CHUNKS * ROWS * 128, KBYTES = CHUNKS * KEYS * 128;
-    static constexpr int V = K + 2 * KBYTES, BAR = V + 2 * KBYTES, SIZE = BAR + 256 + 1024;
+    static constexpr int V = K + 4 * KBYTES, BAR = V + KBYTES, SIZE = BAR + 256;  // keys: two stages of two terms
     static constexpr int THREADS = 288;
     static constexpr uint32_t TMEM = 256;  // O (d columns), two score tiles (64 each)
 };
@@ -53,9 +78,12 @@ struct Tiles {
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
     using L = Tiles<T, D, G>;
+    constexpr bool TWO = std::is_same<T, __half>::value;  // weights in two terms
     constexpr int ROWS = L::ROWS, KEYS = L::KEYS, NG = D / G, TILE = kv4_tile_bytes(D, G);
-    extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+    // no static shared memory here, so that the dynamic one starts on a 1024-byte
+    // boundary, as the operands' swizzle wants it, without room for rounding up:
+    // two blocks fit an SM to within a kilobyte
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::BAR);
     uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8, *p_full = bar + 10,
              *o_done = bar + 12, *q_full = bar + 13;
@@ -190,10 +218,13 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                 }
             }
             // read again rather than held: the weights of columns c, c + 1 go to
-            // column c / 2, over scores that have been read
+            // column c / 2, over scores that have been read, and what rounding
+            // them left (f16 results show it) to column 32 + c / 2, the first
+            // half's once the second has been read
+            uint32_t low[TWO ? 16 : 1];
 #pragma unroll
             for (int c = 0; c < KEYS; c += 32) {
-                uint32_t x[32], p[16];
+                uint32_t x[32], p[16], rest[TWO ? 16 : 1];
                 half(c, x);
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -201,8 +232,21 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                                 v = exp2_fast(fmaf(__uint_as_float(x[2 * i + 1]), c1, -ref));
                     l += u + v;
                     p[i] = pack2(u, v);
+                    if constexpr (TWO) {
+                        const float2 r2 = unpack2(p[i]);
+                        rest[i] = pack2(u - r2.x, v - r2.y);
+                    }
                 }
                 tmem_st16(t_s + lane_base + st * KEYS + c / 2, p);
+                if constexpr (TWO) {
+                    if (c == 0) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) low[i] = rest[i];
+                    } else {
+                        tmem_st16(t_s + lane_base + st * KEYS + 32, low);
+                        tmem_st16(t_s + lane_base + st * KEYS + 48, rest);
+                    }
+                }
             }
             tmem_st_wait();
             tc_fence_before();
@@ -262,16 +306,20 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
             const int tile = (first + j) * 4 + (lane & 3);
             page = tile < n_tiles ? table[quot(tile)] : -1;
         };
-        const auto load = [&](int j) {  // block j's codes to registers
-            const int tile0 = (first + j) * 4, tile = tile0 + (lane & 3);
+        int64_t off = 0, off_v = 0;  // of this lane's tile: of the block whose keys are loaded next, whose values
+        uint32_t have = 0, have_v = 0;
+        const auto place = [&](int j) {  // of block j, whose page has been loaded
+            const int tile = (first + j) * 4 + (lane & 3);
             const bool ok = page >= 0 && page < a.n_pages;
             if (t < 4 && tile < n_tiles && !ok) set_status(a.status, DEV_BAD_ARG);
-            const uint32_t have = __ballot_sync(0xffffffffu, ok) & 15u;
-            there = have | (__ballot_sync(0xffffffffu, tile >= n_tiles) & 15u);
-            const int64_t off = ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + (tile - quot(tile) * page_tiles)) * TILE;
-            const uint8_t *p = a.data + __shfl_sync(0xffffffffu, off, key >> 4), *q = a.data + __shfl_sync(0xffffffffu, off, v_tile);
-            const int r = key & 15;
-            const bool here = have >> (key >> 4) & 1u, v_here = have >> v_tile & 1u;
+            off_v = off, have_v = have;
+            have = __ballot_sync(0xffffffffu, ok) & 15u;
+            off = ((static_cast<int64_t>(page) * a.kv_heads + head) * page_tiles + (tile - quot(tile) * page_tiles)) * TILE;
+        };
+        const auto load_keys = [&](int j) {
+            const int tile0 = (first + j) * 4, r = key & 15;
+            there = have | (__ballot_sync(0xffffffffu, tile0 + (lane & 3) >= n_tiles) & 15u);
+            const uint8_t *p = a.data + __shfl_sync(0xffffffffu, off, key >> 4);
             constexpr int PER = KWORDS / KG;
             if (have != 15u) {
                 asm volatile("");
@@ -279,14 +327,8 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                 for (int i = 0; i < KWORDS; i++) kw[i] = 0;
 #pragma unroll
                 for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < WORDS; w++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) vw[i][w] = 0;
-                    vm[0][2 * w] = vm[0][2 * w + 1] = vm[1][2 * w] = vm[1][2 * w + 1] = 0;
-                }
             }
-            if (here) {
+            if (have >> (key >> 4) & 1u) {
 #pragma unroll
                 for (int g = 0; g < KG; g++) {
                     const int c = c0 + g * (HALF / KG);
@@ -299,7 +341,26 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                     km[g] = reinterpret_cast<const __half2 *>(p + kv4_kmeta(D))[(c / G) * 16 + r];
                 }
             }
-            if (v_here) {
+            if ((tile0 + 4) * 16 > s.len) {  // tokens past the end: whatever their slots hold counts for 0
+                asm volatile("");
+                if (tile0 * 16 + key >= s.len)
+#pragma unroll
+                    for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
+            }
+        };
+        const auto load_values = [&](int j, int64_t o, uint32_t h) {
+            const int tile0 = (first + j) * 4;
+            const uint8_t *q = a.data + __shfl_sync(0xffffffffu, o, v_tile);
+            if (h != 15u) {
+                asm volatile("");
+#pragma unroll
+                for (int w = 0; w < WORDS; w++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) vw[i][w] = 0;
+                    vm[0][2 * w] = vm[0][2 * w + 1] = vm[1][2 * w] = vm[1][2 * w + 1] = 0;
+                }
+            }
+            if (h >> v_tile & 1u) {
                 const uint8_t *codes = q + kv4_val(D) + oct * 64 + 4 * j0;
                 const uint8_t *meta = q + kv4_vmeta(D, G) + ((oct * 8 / G) * 16 + 2 * j0) * 4;
 #pragma unroll
@@ -307,11 +368,8 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) memcpy(vm[i], __builtin_assume_aligned(meta + 32 * i, 8 * WORDS), 8 * WORDS);
             }
-            if ((tile0 + 4) * 16 > s.len) {  // tokens past the end: whatever their slots hold counts for 0
+            if ((tile0 + 4) * 16 > s.len) {
                 asm volatile("");
-                if (tile0 * 16 + key >= s.len)
-#pragma unroll
-                    for (int g = 0; g < KG; g++) km[g] = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -319,26 +377,41 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                         if ((tile0 + v_tile) * 16 + 2 * j0 + 8 * i + k >= s.len) vm[i][k] = 0;
             }
         };
-        if (n > 0) {
-            find(0);
-            load(0);
-            if (n > 1) find(1);
-        }
-        for (int j = 0; j < n; j++) {
+        const auto expand_keys = [&](int j) {
             const int st = j & 1;
-            uint8_t *ks = smem + L::K + st * L::KBYTES, *vs = smem + L::V + st * L::KBYTES;
+            uint8_t *ks = smem + L::K + st * 2 * L::KBYTES;
             if (j >= 2) wait(&k_empty[st], (j >> 1) - 1 & 1);
             if (t == 0) oks[j & 3] = there;
 #pragma unroll
             for (int i = 0; i < KWORDS; i++) {
                 const __half2 m = km[i / (KWORDS / KG)];
-                const int c = c0 / 8 + i;
-                *reinterpret_cast<uint4 *>(ks + c / 8 * (KEYS * 128) + sw128_offset(key, c % 8)) =
-                    kv4_expand(kw[i], __low2half2(m), __high2half2(m));
+                const int c = c0 / 8 + i, at = c / 8 * (KEYS * 128) + sw128_offset(key, c % 8);
+                uint4 high, low;
+                kv4_expand2(kw[i], __low2half2(m), __high2half2(m), high, low);
+                *reinterpret_cast<uint4 *>(ks + at) = high;
+                *reinterpret_cast<uint4 *>(ks + L::KBYTES + at) = low;
             }
             fence_proxy_async_smem();
             mbar_arrive(&k_full[st]);
-            if (j >= 2) wait(&v_empty[st], (j >> 1) - 1 & 1);
+        };
+        // Keys go a block ahead of values, which have one stage.
+        if (n > 0) {
+            find(0);
+            place(0);
+            load_keys(0);
+            if (n > 1) find(1);
+            load_values(0, off, have);
+            expand_keys(0);
+            if (n > 1) {
+                place(1);
+                load_keys(1);
+                if (n > 2) find(2);
+            }
+        }
+        for (int j = 0; j < n; j++) {
+            if (j + 1 < n) expand_keys(j + 1);
+            uint8_t *vs = smem + L::V;
+            if (j >= 1) wait(v_empty, j - 1 & 1);
 #pragma unroll
             for (int w = 0; w < WORDS; w++) {
                 // four pairs' bytes of four tokens -> four tokens' eight channels
@@ -355,10 +428,14 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                 }
             }
             fence_proxy_async_smem();
-            mbar_arrive(&v_full[st]);
+            mbar_arrive(v_full);
             if (j + 1 < n) {
-                load(j + 1);
-                if (j + 2 < n) find(j + 2);
+                if (j + 2 < n) place(j + 2);
+                load_values(j + 1, j + 2 < n ? off_v : off, j + 2 < n ? have_v : have);
+                if (j + 2 < n) {
+                    load_keys(j + 2);
+                    if (j + 3 < n) find(j + 3);
+                }
             }
         }
     } else if (tid == 256 && n > 0) {
@@ -370,10 +447,12 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
             tc_fence_after();
             if (!dead)
 #pragma unroll
-                for (int kk = 0; kk < D / 16; kk++)
-                    umma_f16(t_s + st * KEYS, sdesc_sw128(qa + (kk >> 2) * (ROWS * 128) + (kk & 3) * 32, 16, 1024),
-                             sdesc_sw128(ka + st * L::KBYTES + (kk >> 2) * (KEYS * 128) + (kk & 3) * 32, 16, 1024), id_s,
-                             kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < 2 * (D / 16); kk++) {  // the low terms, then the high ones
+                    const int k = kk % (D / 16), term = kk < D / 16 ? 1 : 0;
+                    umma_f16(t_s + st * KEYS, sdesc_sw128(qa + (k >> 2) * (ROWS * 128) + (k & 3) * 32, 16, 1024),
+                             sdesc_sw128(ka + (2 * st + term) * L::KBYTES + (k >> 2) * (KEYS * 128) + (k & 3) * 32, 16, 1024),
+                             id_s, kk > 0 ? 1u : 0u);
+                }
             umma_commit(&s_full[st]);
             umma_commit(&k_empty[st]);
         };
@@ -382,16 +461,16 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
         for (int j = 0; j < n; j++) {
             const int st = j & 1;
             if (j + 1 < n) scores(j + 1);
-            wait(&v_full[st], j >> 1 & 1);
+            wait(v_full, j & 1);
             wait(&p_full[st], j >> 1 & 1);
             tc_fence_after();
             if (!dead)
 #pragma unroll
-                for (int kk = 0; kk < KEYS / 16; kk++)
+                for (int kk = 0; kk < (TWO ? 2 : 1) * (KEYS / 16); kk++)
                     umma_f16_ts(t_o, t_s + st * KEYS + 8 * kk,
-                                sdesc_make(va + st * L::KBYTES + kk * 2048, KEYS * 128, 1024, LAYOUT_SW128), id_o,
+                                sdesc_make(va + kk % (KEYS / 16) * 2048, KEYS * 128, 1024, LAYOUT_SW128), id_o,
                                 j > 0 || kk > 0 ? 1u : 0u);
-            umma_commit(&v_empty[st]);
+            umma_commit(v_empty);
             umma_commit(o_done);
         }
         wait(o_done, (n - 1) & 1);
