@@ -790,19 +790,19 @@ st_status launch(st_handle *h, AttnArgs a) {
 
 // Whether rows of 16-bit types go by tiles of 128 (with a positive scale: the
 // largest score is the largest product).  A tile goes through its keys alone,
-// so it takes many tiles, or few keys, to be ahead of the kernel that cuts
-// the keys for all teams.  Both as measured, in us: a block of 64 keys takes a tile
-// 1.15 where it has its SM alone and 1.75 where two share one; the teams
-// together do 785 steps of 32 keys and 16 rows a us (1300 at d = 64) after a start of
-// 14.  E.g. 32 heads on 8, d 128: one sequence of 8192 keys, 128 rows 149 by tiles
-// and 96 by teams, 256 rows 148 and 175, 1024 rows 211 and 668; 16 sequences of
-// 4096, 8 rows each 80 and 56, 16 rows 80 and 99.
+// so it takes many tiles, or few keys, to be ahead of the kernel that cuts the
+// keys for all teams.  Both as measured, in us: a block of 64 keys takes a tile
+// 1.65 where it has its SM alone and 2.35 where two share one; the teams
+// together do 785 steps of 32 keys and 16 rows a us (1300 at d = 64) after a start
+// of 14.  E.g. 32 heads on 8, d 128: one sequence of 8192 keys, 128 queries 212 by
+// tiles and 95 by teams, 256 213 and 176, 1024 290 and 670; 16 sequences of 4096
+// keys, 16 queries each 113 and 99, 32 115 and 186.
 bool by_tiles(const AttnArgs &a) {
     const int64_t rows = a.max_q * static_cast<int64_t>(a.share), keys = a.max_pages * a.page;
     if (a.scale_log2 <= 0.0f || rows <= 16 || a.batch > 65535) return false;
     const double seqs = static_cast<double>(a.batch) * a.kv_heads;
     const double tiles = seqs * static_cast<double>((rows + 127) / 128);
-    const double by_tile = 5.0 + keys / 64.0 * (tiles <= a.sms ? 1.15 : 1.75 * std::ceil(tiles / (2.0 * a.sms)));
+    const double by_tile = 5.0 + keys / 64.0 * (tiles <= a.sms ? 1.65 : 2.35 * std::ceil(tiles / (2.0 * a.sms)));
     const double steps = seqs * static_cast<double>((rows + 15) / 16) * (keys / 32.0);
     return by_tile < 14.0 + steps / (a.d == 128 ? 785.0 : 1300.0);
 }

@@ -460,6 +460,9 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
         scores(0);
         for (int j = 0; j < n; j++) {
             const int st = j & 1;
+            // products of different shapes may pass one another: the next scores go
+            // over weights that the product before this one has read
+            if (j + 1 < n && j > 0) wait(o_done, (j - 1) & 1);
             if (j + 1 < n) scores(j + 1);
             wait(v_full, j & 1);
             wait(&p_full[st], j >> 1 & 1);

@@ -194,6 +194,7 @@ TILED = [
     ([700, 20, 511], [500, 450, 1], 12, 2, 64, 64, 32, True, 0, False),
     ([333, 900], [333, 640], 7, 1, 64, 32, 128, False, 0, True),
     ([1200], [600], 5, 5, 128, 64, 16, False, 200, False),
+    ([300, 290, 280, 310, 150], [300, 290, 280, 310, 150], 12, 3, 64, 32, 16, True, 0, False),
 ]
 
 
@@ -211,10 +212,28 @@ def test_attend_by_tiles(dev, case, aligned):
     kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV)
     args = dict(q_start=start, max_q=max(counts), causal=causal, one=one, window=window)
     o = kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **args)
-    assert dev.last_kernel == "k_kv4_attn_tiles" or case == 5  # few heads and keys: either kernel
+    assert dev.last_kernel == "k_kv4_attn_tiles" or case in (4, 5)  # few heads and keys: either kernel
     want, _, vmax = attend64(q, data, pages, lens, counts, d ** -0.5, group, causal, window, one)
     close(o, want, vmax, BF16)
     assert torch.equal(o, kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **args))
+    dev.sync()
+
+
+@pytest.mark.parametrize("case", [0, 1, 2, 3, 6])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attend_by_tiles_with_lse(dev, case, dtype):
+    lens, counts, heads, kv_heads, d, group, page, causal, window, one = TILED[case]
+    data, pages = filled(lens, kv_heads, d, group, page, 70 + case)
+    g = torch.Generator(device=DEV).manual_seed(case)
+    q = (torch.randn((sum(counts), heads, d), generator=g, device=DEV) * 2).to(dtype)
+    start = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o, lse = kv4().attend(q, data, pages, kv_len, d ** -0.5, group, q_start=start, max_q=max(counts), causal=causal,
+                          one=one, window=window, return_lse=True)
+    assert dev.last_kernel == "k_kv4_attn_tiles"
+    want, want_lse, vmax = attend64(q, data, pages, lens, counts, d ** -0.5, group, causal, window, one)
+    close(o, want, vmax, dtype)
+    close_lse(lse, want_lse, dtype)
     dev.sync()
 
 
