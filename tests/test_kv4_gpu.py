@@ -219,6 +219,27 @@ def test_attend_by_tiles(dev, case, aligned):
     dev.sync()
 
 
+@pytest.mark.parametrize("case", [2, 5])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attend_by_tiles_from_a_cold_cache(dev, case, dtype):
+    """Two or three blocks of keys a tile, far from the chip: values come late, and the last product later than scores."""
+    lens, counts, heads, kv_heads, d, group, page, causal, window, one = TILED[case]
+    data, pages = filled(lens, kv_heads, d, group, page, 80 + case)
+    g = torch.Generator(device=DEV).manual_seed(case)
+    q = (torch.randn((sum(counts), heads, d), generator=g, device=DEV) * 2).to(dtype)
+    start = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    args = dict(q_start=start, max_q=max(counts), causal=causal, one=one, window=window)
+    flush, outs = torch.empty(1 << 28, dtype=torch.uint8, device=DEV), []
+    for i in range(40):
+        flush.fill_(i)
+        outs.append(kv4().attend(q, data, pages, kv_len, d ** -0.5, group, **args))
+    want, _, vmax = attend64(q, data, pages, lens, counts, d ** -0.5, group, causal, window, one)
+    close(outs[0], want, vmax, dtype)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    dev.sync()
+
+
 @pytest.mark.parametrize("case", [0, 1, 2, 3, 6])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_attend_by_tiles_with_lse(dev, case, dtype):
