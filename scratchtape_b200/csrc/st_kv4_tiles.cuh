@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::BAR);
     uint64_t *k_full = bar, *k_empty = bar + 2, *s_full = bar + 4, *p_full = bar + 6, *v_full = bar + 8, *o_done = bar + 9,
-             *q_full = bar + 10;
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 11), *oks = tslot + 4;  // oks[4]: tiles that are there, by block % 4
+             *q_full = bar + 10, *all_done = bar + 11;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(bar + 12), *oks = tslot + 4;  // oks[4]: tiles that are there, by block % 4
     const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
         }
         mbar_init(v_full, 128);
         mbar_init(o_done, 1);
+        mbar_init(all_done, 1);
         mbar_init(q_full, 128);
         fence_mbar_init();
     }
@@ -260,9 +261,8 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
             tc_fence_before();
             mbar_arrive(&p_full[st]);
         }
-        // one phase after the other: a wait tells a phase from the next, not from the one after
-        if (n > 1) wait_all(o_done, (n - 2) & 1);
-        if (n > 0) wait_all(o_done, (n - 1) & 1);
+        // a barrier of its own: o_done may be one or two phases behind here, and parity tells only one of them
+        if (n > 0) wait_all(all_done, 0);
         tc_fence_after();
         float top = ref, sum = l, fix = 1.0f;
         if (a.one) {
@@ -488,8 +488,8 @@ __global__ void __launch_bounds__(288, 2) k_kv4_attn_tiles(const AttnArgs a) {
                                 j > 0 || kk > 0 ? 1u : 0u);
             umma_commit(o_done);
         }
-        if (n > 1) wait(o_done, (n - 2) & 1);
-        wait(o_done, (n - 1) & 1);
+        umma_commit(all_done);
+        wait(all_done, 0);
     }
     __syncwarp();
     tc_fence_before();
