@@ -1,7 +1,7 @@
 /*
  * st_b200.h -- C ABI of scratchtape-b200, the B200 (sm_100a) implementation
  * of scratchtape's matmul family, batched causal attention and 2-bit kNN
- * scoring.
+ * scoring, and of token generation over a 4-bit cache.
  *
  * Conventions
  *  - Every call enqueues on the handle's CUDA stream and returns at once; no

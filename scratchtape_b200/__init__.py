@@ -2,7 +2,8 @@
 
 The package is a thin host layer over ``libst_b200.so`` (C ABI in
 ``include/st_b200.h``): the matmul family, row softmax, fused causal
-attention and 2-bit kNN scoring.  Importing it without the built library
+attention, 2-bit kNN scoring, and token generation over a 4-bit cache
+(``kv4``, ``logits``, ``generate``).  Importing it without the built library
 fails; there is no CPU fallback.
 """
 from . import _native  # noqa: F401  (fails loudly when the library is missing)

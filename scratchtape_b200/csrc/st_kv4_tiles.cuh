@@ -9,7 +9,7 @@
 // weights and put them back into the same TMEM columns as the A operand of the
 // second product.  Two blocks share an SM, so one's products run while the
 // other's softmax does.  2,100 rows of up to 8192 keys, 32 heads on 8 of 128, bf16:
-// 524 us, a quarter of the bf16 rate; bound by a block's own chain of
+// 534 us, a quarter of the bf16 rate; bound by a block's own chain of
 // expansion, product, softmax and product, 3100 cycles for 64 keys.
 //
 // Roundings: queries are exact in f16 (a power of two per row), keys in two terms

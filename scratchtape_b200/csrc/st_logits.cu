@@ -104,7 +104,8 @@ __device__ __forceinline__ void mask_row(const LogitsArgs &a, int64_t r, const u
 }
 
 // All of the rows but for the tokens that k_logits_tokens adjusts afterwards:
-// a copy, -inf where the mask has a 0.  Bound by memory.
+// a copy, -inf where the mask has a 0.  Bound by memory: 256 x 131,075 bf16 in
+// 27.8 us, 4.9 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(MASK_THREADS) k_logits_mask(const LogitsArgs a) {
     grid_dep_wait();
@@ -118,7 +119,9 @@ __global__ void __launch_bounds__(MASK_THREADS) k_logits_mask(const LogitsArgs a
 // place.  Up to HASHED entries go through a hash table of SLOTS by one block;
 // longer histories are looked through by a block for each WINDOW of the
 // vocabulary, which counts it densely.  With one window the block has copied
-// its row itself.
+// its row itself.  Bound by latency: shared atomics, then scattered logits; 256
+// rows of up to 4096 tokens take 25 us after the mask's 28.  (One launch that
+// counted for each 16,384 tokens of the vocabulary anew took 61 in all.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS) k_logits_tokens(const LogitsArgs a, int after_mask) {
     constexpr int VEC = 16 / sizeof(T), BATCH = 8;
